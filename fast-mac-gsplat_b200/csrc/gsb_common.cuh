@@ -22,6 +22,7 @@ enum ErrorSite : uint32_t {
   kSiteScanTotal = 6,
   kSitePeerStart = 7,
   kSitePeerEnd = 8,
+  kSiteCode = 9,
 };
 
 // Raster configuration passed to kernels by value (no device meta tensors, no

@@ -21,6 +21,7 @@
 
 #include <array>
 #include <cstdlib>
+#include <cstring>
 #include <map>
 #include <mutex>
 #include <optional>
@@ -155,6 +156,60 @@ struct ErrorRing {
 ErrorRing& errors() {
   static ErrorRing* r = new ErrorRing();
   return *r;
+}
+
+// Status blocks of the codebook ops, one per device, in pinned host memory that
+// the kernels write through its mapping: an op needs no copy, event or side
+// stream for its errors, so it can be captured into a graph whose replays report
+// theirs too. Read by the next codebook op of the device and by
+// check_device_errors().
+struct MappedStatus {
+  static constexpr int kMaxDevices = 64;
+  std::mutex mu;
+  volatile uint32_t* words = nullptr;  // [kMaxDevices][GSB_STATUS_WORDS]
+  std::array<bool, kMaxDevices> used{};
+
+  uint32_t* of(int dev) {
+    if (dev < 0 || dev >= kMaxDevices) throw std::runtime_error("gsplat_b200: device index out of range");
+    std::lock_guard<std::mutex> g(mu);
+    if (words == nullptr) {
+      // The allocation is no stream operation; it must not end a capture in progress.
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      void* p = nullptr;
+      const size_t bytes = sizeof(uint32_t) * kMaxDevices * GSB_STATUS_WORDS;
+      const cudaError_t e = cudaHostAlloc(&p, bytes, cudaHostAllocPortable | cudaHostAllocMapped);
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      if (e != cudaSuccess) throw std::runtime_error("gsplat_b200: no pinned host memory for the status blocks");
+      std::memset(p, 0, bytes);
+      words = static_cast<volatile uint32_t*>(p);
+    }
+    used[dev] = true;
+    return const_cast<uint32_t*>(words) + dev * GSB_STATUS_WORDS;  // unified addressing: the device's address too
+  }
+  // Raises, once, an error that a finished kernel of the device has recorded.
+  void check(int dev) {
+    if (words == nullptr) return;
+    volatile uint32_t* w = words + dev * GSB_STATUS_WORDS;
+    const uint32_t flags = w[GSB_STATUS_ERROR];
+    if (!flags) return;
+    const uint32_t site = w[GSB_STATUS_ERROR_SITE];
+    w[GSB_STATUS_ERROR] = 0;
+    w[GSB_STATUS_ERROR_SITE] = 0;
+    throw std::runtime_error(decode_device_error(flags, site));
+  }
+  void check_all() {
+    for (int d = 0; d < kMaxDevices; ++d) {
+      if (!used[d]) continue;
+      const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(d));
+      C10_CUDA_CHECK(cudaDeviceSynchronize());
+      check(d);
+    }
+  }
+};
+MappedStatus& mapped_status() {
+  static MappedStatus* m = new MappedStatus();
+  return *m;
 }
 
 // Optional per-phase CUDA-event timing (bench instrumentation): events bracket
@@ -678,7 +733,251 @@ std::tuple<Tensor, Tensor, Tensor> op_sh_bwd(const Tensor& sh, const Tensor& mea
   return {g_sh, g_m, g_k};
 }
 
-void check_device_errors() { errors().check_all(nullptr); }
+// ---- codebook attributes (no reference counterpart) -------------------------
+
+int32_t code_dtype(const Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return GSB_DTYPE_F32;
+    case at::kBFloat16: return GSB_DTYPE_BF16;
+    case at::kHalf: return GSB_DTYPE_F16;
+    default: value_error(std::string("gsplat_b200: ") + name + " must be float32, bfloat16 or float16");
+  }
+}
+
+void check_same_device(const Tensor& t, const Tensor& like, const char* name) {
+  if (!t.is_cuda() || t.device() != like.device())
+    value_error(std::string("gsplat_b200: ") + name + " must be on the same CUDA device");
+}
+
+Tensor code_tensor(const Tensor& codes, const Tensor& like) {
+  check_same_device(codes, like, "codes");
+  if (codes.scalar_type() != at::kInt && codes.scalar_type() != at::kLong)
+    value_error("gsplat_b200: codes must be int32 or int64");
+  return codes.contiguous();
+}
+
+int32_t code_bytes(const Tensor& codes) { return codes.scalar_type() == at::kLong ? 8 : 4; }
+
+// A status block for the op's kernels; raises what earlier ones have recorded.
+uint32_t* codebook_status(const Tensor& t) {
+  const int dev = t.device().index();
+  uint32_t* s = mapped_status().of(dev);
+  mapped_status().check(dev);
+  return s;
+}
+// Under GSPLAT_B200_CHECK the op waits for its own errors (not in a capture).
+void codebook_done(const Tensor& t) {
+  if (!debug_checks()) return;
+  const auto cur = at::cuda::getCurrentCUDAStream(t.device().index());
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  C10_CUDA_CHECK(cudaStreamIsCapturing(cur.stream(), &capturing));
+  if (capturing != cudaStreamCaptureStatusNone) return;
+  cur.synchronize();
+  mapped_status().check(t.device().index());
+}
+
+// Rows of contiguous values at any row stride: [C, ...] as [C, dim], [..., C] as [rows, C].
+Tensor table_rows(const Tensor& table) {
+  if (table.dim() < 1 || table.size(0) < 1 || table.numel() == 0)
+    value_error("gsplat_b200: codebook must be [C,...] with at least one row and value");
+  Tensor t = table.dim() == 1 ? table.unsqueeze(1) : table.flatten(1);
+  return t.stride(1) == 1 || t.size(1) == 1 ? t : t.contiguous();
+}
+Tensor logit_rows(const Tensor& logits) {
+  if (logits.dim() < 1 || logits.size(-1) < 1) value_error("gsplat_b200: logits must be [...,C] with at least one code");
+  const int64_t C = logits.size(-1);
+  Tensor t = logits.numel() == 0 ? logits.new_empty({0, C}) : logits.reshape({-1, C});
+  return t.stride(1) == 1 || C == 1 ? t : t.contiguous();
+}
+
+struct LookupShape {
+  int64_t rows, bag;
+  std::vector<int64_t> out;
+};
+LookupShape lookup_shape(const Tensor& codebook, const Tensor& codes, const std::optional<Tensor>& weights) {
+  LookupShape s;
+  s.out = codes.sizes().vec();
+  s.bag = 1;
+  if (weights.has_value() && weights->defined()) {
+    check_same_device(*weights, codebook, "weights");
+    if (weights->scalar_type() != at::kFloat) value_error("gsplat_b200: weights must be float32");
+    if (codes.dim() < 1 || weights->sizes() != codes.sizes() || codes.size(-1) < 1)
+      value_error("gsplat_b200: weights must have the shape [...,J] of codes");
+    s.bag = codes.size(-1);
+    s.out.pop_back();
+  }
+  s.rows = codes.numel() / s.bag;
+  const auto row = codebook.sizes().slice(1);
+  s.out.insert(s.out.end(), row.begin(), row.end());
+  return s;
+}
+
+// Rows of a codebook by code -> [..., *row] (weighted sums over the last axis of codes, with weights).
+Tensor op_codebook_fwd(const Tensor& codebook, const Tensor& codes, const std::optional<Tensor>& weights, double scale,
+                       at::ScalarType out_dtype) {
+  const int32_t dt = code_dtype(codebook, "codebook");
+  const c10::cuda::CUDAGuard guard(codebook.device());
+  const LookupShape shape = lookup_shape(codebook, codes, weights);
+  const Tensor t = table_rows(codebook), c = code_tensor(codes, codebook);
+  const Tensor w = weights.has_value() && weights->defined() ? weights->contiguous() : Tensor();
+  uint32_t* status = codebook_status(t);
+  Tensor out = empty(shape.out, out_dtype, t.device());
+  check(gsb_codebook_forward(dt, code_dtype(out, "out_dtype"), shape.rows, static_cast<int32_t>(shape.bag), t.size(0),
+                             static_cast<int32_t>(t.size(1)), t.data_ptr(), t.stride(0), c.data_ptr(), code_bytes(c),
+                             ptr<float>(w), static_cast<float>(scale), out.data_ptr(), status, stream_of(t)),
+        "gsb_codebook_forward");
+  codebook_done(t);
+  return out;
+}
+
+std::tuple<Tensor, Tensor> op_codebook_bwd(const Tensor& grad_out, const Tensor& codebook, const Tensor& codes,
+                                           const std::optional<Tensor>& weights, double scale, bool need_codebook,
+                                           bool need_weights) {
+  const int32_t dt = code_dtype(codebook, "codebook");
+  check_same_device(grad_out, codebook, "grad_out");
+  const c10::cuda::CUDAGuard guard(codebook.device());
+  const LookupShape shape = lookup_shape(codebook, codes, weights);
+  if (grad_out.sizes() != at::IntArrayRef(shape.out)) value_error("gsplat_b200: grad_out has another shape");
+  const Tensor t = table_rows(codebook), c = code_tensor(codes, codebook), g = grad_out.contiguous();
+  const Tensor w = weights.has_value() && weights->defined() ? weights->contiguous() : Tensor();
+  uint32_t* status = codebook_status(t);
+  Tensor g_table, g_w, ws;
+  size_t ws_bytes = 0;
+  if (need_codebook) {
+    g_table = empty(codebook.sizes(), codebook.scalar_type(), t.device());
+    ws_bytes = gsb_codebook_backward_workspace_size(shape.rows, static_cast<int32_t>(shape.bag), t.size(0),
+                                                    static_cast<int32_t>(t.size(1)));
+    ws = empty({static_cast<int64_t>(std::max<size_t>(ws_bytes, 1))}, at::kByte, t.device());
+  }
+  if (need_weights && w.defined()) g_w = empty(w.sizes(), at::kFloat, t.device());
+  if (g_table.defined() || g_w.defined()) {
+    check(gsb_codebook_backward(dt, code_dtype(g, "grad_out"), shape.rows, static_cast<int32_t>(shape.bag), t.size(0),
+                                static_cast<int32_t>(t.size(1)), t.data_ptr(), t.stride(0), c.data_ptr(),
+                                code_bytes(c), ptr<float>(w), static_cast<float>(scale), g.data_ptr(),
+                                g_table.defined() ? g_table.data_ptr() : nullptr, ptr<float>(g_w), status,
+                                ws.defined() ? ws.data_ptr() : nullptr, ws_bytes, stream_of(t)),
+          "gsb_codebook_backward");
+    codebook_done(t);
+  }
+  return {g_table, g_w};
+}
+
+std::vector<int64_t> lead_shape(const Tensor& logits) {
+  std::vector<int64_t> s = logits.sizes().vec();
+  s.pop_back();
+  return s;
+}
+
+// -> log_probs [...] (undefined without codes), entropy [...], top_log_probs and top_codes [...,top_k],
+// stats [rows,4] (undefined unless save_state).
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> op_code_log_probs_fwd(const Tensor& logits,
+                                                                         const std::optional<Tensor>& codes,
+                                                                         int64_t top_k, bool save_state) {
+  const int32_t dt = code_dtype(logits, "logits");
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const at::Device dev = logits.device();
+  const Tensor z = logit_rows(logits);
+  const std::vector<int64_t> lead = lead_shape(logits);
+  std::vector<int64_t> topped = lead;
+  topped.push_back(top_k);
+  if (top_k < 0 || top_k > GSB_CODE_MAX_TOP || top_k > z.size(1))
+    value_error("gsplat_b200: top_k must be 0.." + std::to_string(GSB_CODE_MAX_TOP) + " and at most the codes");
+  Tensor c, lp, stats;
+  if (codes.has_value() && codes->defined()) {
+    if (codes->sizes() != at::IntArrayRef(lead)) value_error("gsplat_b200: codes must have the shape [...] of logits");
+    c = code_tensor(*codes, logits);
+    lp = empty(lead, at::kFloat, dev);
+  }
+  uint32_t* status = codebook_status(z);
+  Tensor ent = empty(lead, at::kFloat, dev), tl = empty(topped, at::kFloat, dev), tc = empty(topped, at::kInt, dev);
+  if (save_state) stats = empty({z.size(0), 4}, at::kFloat, dev);
+  check(gsb_code_log_probs_forward(dt, z.size(0), z.size(1), z.data_ptr(), z.stride(0),
+                                   c.defined() ? c.data_ptr() : nullptr, c.defined() ? code_bytes(c) : 4,
+                                   static_cast<int32_t>(top_k), ptr<float>(lp), ptr<float>(ent), ptr<float>(tl),
+                                   ptr<int32_t>(tc), ptr<float>(stats), status, stream_of(z)),
+        "gsb_code_log_probs_forward");
+  codebook_done(z);
+  return {lp, ent, tl, tc, stats};
+}
+
+Tensor opt_f32(const std::optional<Tensor>& g) {
+  if (!g.has_value() || !g->defined()) return Tensor();
+  return g->to(at::kFloat).contiguous();
+}
+
+Tensor op_code_log_probs_bwd(const std::optional<Tensor>& g_log_probs, const std::optional<Tensor>& g_entropy,
+                             const std::optional<Tensor>& g_top, const Tensor& logits,
+                             const std::optional<Tensor>& codes, const Tensor& top_codes, const Tensor& stats) {
+  const int32_t dt = code_dtype(logits, "logits");
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const Tensor z = logit_rows(logits);
+  const Tensor gl = opt_f32(g_log_probs), gh = opt_f32(g_entropy), gt = opt_f32(g_top);
+  const Tensor c = codes.has_value() && codes->defined() ? code_tensor(*codes, logits) : Tensor();
+  const Tensor tc = top_codes.contiguous();
+  const int64_t rows = z.size(0), top_k = tc.size(-1);
+  auto has = [&](const Tensor& t, int64_t n) { return !t.defined() || (t.is_cuda() && t.numel() == n); };
+  if (!has(gl, rows) || !has(gh, rows) || !has(gt, rows * top_k) || !has(c, rows) || tc.numel() != rows * top_k ||
+      tc.scalar_type() != at::kInt || stats.numel() != rows * 4 || stats.scalar_type() != at::kFloat)
+    value_error("gsplat_b200: the gradients do not match the forward's outputs");
+  Tensor dz = empty(logits.sizes(), logits.scalar_type(), z.device());
+  check(gsb_code_log_probs_backward(dt, rows, z.size(1), z.data_ptr(), z.stride(0),
+                                    c.defined() ? c.data_ptr() : nullptr, c.defined() ? code_bytes(c) : 4,
+                                    static_cast<int32_t>(top_k), ptr<int32_t>(tc), ptr<float>(stats.contiguous()),
+                                    ptr<float>(gl), ptr<float>(gh), ptr<float>(gt), dz.data_ptr(), stream_of(z)),
+        "gsb_code_log_probs_backward");
+  return dz;
+}
+
+// -> loss [], counts [C], stats [rows,4] (undefined unless save_state), coef [1].
+std::tuple<Tensor, Tensor, Tensor, Tensor> op_code_balance_fwd(const Tensor& logits, const Tensor& codes,
+                                                               bool save_state) {
+  const int32_t dt = code_dtype(logits, "logits");
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const at::Device dev = logits.device();
+  const Tensor z = logit_rows(logits), c = code_tensor(codes, logits);
+  const int64_t rows = z.size(0), C = z.size(1);
+  std::vector<int64_t> lead = lead_shape(logits), given = codes.sizes().vec();
+  int64_t bag = 1;
+  if (given.size() == lead.size() + 1) {
+    bag = given.back();
+    given.pop_back();
+  }
+  if (given != lead || bag < 1) value_error("gsplat_b200: codes must have the shape [...] or [...,J] of logits");
+  uint32_t* status = codebook_status(z);
+  Tensor loss = empty({}, at::kFloat, dev), counts = empty({C}, at::kInt, dev), coef = empty({1}, at::kFloat, dev);
+  Tensor stats;
+  if (save_state) stats = empty({rows, 4}, at::kFloat, dev);
+  const size_t ws_bytes = gsb_code_balance_workspace_size(rows, C);
+  Tensor ws = empty({static_cast<int64_t>(std::max<size_t>(ws_bytes, 1))}, at::kByte, dev);
+  check(gsb_code_balance_forward(dt, rows, C, static_cast<int32_t>(bag), z.data_ptr(), z.stride(0), c.data_ptr(),
+                                 code_bytes(c), ptr<float>(loss), ptr<int32_t>(counts), ptr<float>(stats),
+                                 ptr<float>(coef), status, ws.data_ptr(), ws_bytes, stream_of(z)),
+        "gsb_code_balance_forward");
+  codebook_done(z);
+  return {loss, counts, stats, coef};
+}
+
+Tensor op_code_balance_bwd(const Tensor& g_loss, const Tensor& logits, const Tensor& counts, const Tensor& stats,
+                           const Tensor& coef) {
+  const int32_t dt = code_dtype(logits, "logits");
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const Tensor z = logit_rows(logits), g = g_loss.to(at::kFloat).contiguous();
+  check_same_device(g, logits, "g_loss");
+  if (g.numel() != 1 || coef.numel() != 1 || counts.numel() != z.size(1) || counts.scalar_type() != at::kInt ||
+      stats.numel() != z.size(0) * 4 || stats.scalar_type() != at::kFloat)
+    value_error("gsplat_b200: the gradient does not match the forward's outputs");
+  Tensor dz = empty(logits.sizes(), logits.scalar_type(), z.device());
+  check(gsb_code_balance_backward(dt, z.size(0), z.size(1), z.data_ptr(), z.stride(0),
+                                  ptr<int32_t>(counts.contiguous()), ptr<float>(stats.contiguous()), ptr<float>(coef),
+                                  ptr<float>(g), dz.data_ptr(), stream_of(z)),
+        "gsb_code_balance_backward");
+  return dz;
+}
+
+void check_device_errors() {
+  errors().check_all(nullptr);
+  mapped_status().check_all();
+}
 
 void set_phase_timing(bool on) {
   std::lock_guard<std::mutex> g(phase_timer().mu);
@@ -726,6 +1025,16 @@ TORCH_LIBRARY(gsplat_b200, m) {
   m.def("sh_fwd(Tensor sh_coeffs, Tensor means3d, Tensor camera_to_world, int degree) -> Tensor");
   m.def("sh_bwd(Tensor sh_coeffs, Tensor means3d, Tensor camera_to_world, Tensor colors, Tensor grad_colors, "
         "int degree, bool need_means3d, bool need_camera_to_world) -> (Tensor, Tensor, Tensor)");
+  m.def("codebook_fwd(Tensor codebook, Tensor codes, Tensor? weights, float scale, ScalarType out_dtype) -> Tensor");
+  m.def("codebook_bwd(Tensor grad_out, Tensor codebook, Tensor codes, Tensor? weights, float scale, "
+        "bool need_codebook, bool need_weights) -> (Tensor, Tensor)");
+  m.def("code_log_probs_fwd(Tensor logits, Tensor? codes, int top_k, bool save_state) -> (Tensor log_probs, "
+        "Tensor entropy, Tensor top_log_probs, Tensor top_codes, Tensor stats)");
+  m.def("code_log_probs_bwd(Tensor? g_log_probs, Tensor? g_entropy, Tensor? g_top_log_probs, Tensor logits, "
+        "Tensor? codes, Tensor top_codes, Tensor stats) -> Tensor");
+  m.def("code_balance_fwd(Tensor logits, Tensor codes, bool save_state) -> (Tensor loss, Tensor counts, Tensor stats, "
+        "Tensor coef)");
+  m.def("code_balance_bwd(Tensor g_loss, Tensor logits, Tensor counts, Tensor stats, Tensor coef) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(gsplat_b200, CUDA, m) {
@@ -738,6 +1047,12 @@ TORCH_LIBRARY_IMPL(gsplat_b200, CUDA, m) {
   m.impl("project_bwd", &op_project_bwd);
   m.impl("sh_fwd", &op_sh_fwd);
   m.impl("sh_bwd", &op_sh_bwd);
+  m.impl("codebook_fwd", &op_codebook_fwd);
+  m.impl("codebook_bwd", &op_codebook_bwd);
+  m.impl("code_log_probs_fwd", &op_code_log_probs_fwd);
+  m.impl("code_log_probs_bwd", &op_code_log_probs_bwd);
+  m.impl("code_balance_fwd", &op_code_balance_fwd);
+  m.impl("code_balance_bwd", &op_code_balance_bwd);
 }
 
 PYBIND11_MODULE(_gsb_host, m) {

@@ -12,6 +12,7 @@ from .rasterize import (
     rasterize_pinhole_gaussians,
     rasterize_projected_gaussians,
 )
+from .codebook import CodeBalance, CodeLogProbs, code_balance_loss, code_log_probs, codebook_lookup
 from .sh import spherical_harmonics_colors
 
 __all__ = [
@@ -24,4 +25,9 @@ __all__ = [
     "rasterize_projected_gaussians",
     "profile_projected_gaussians",
     "spherical_harmonics_colors",
+    "codebook_lookup",
+    "code_log_probs",
+    "CodeLogProbs",
+    "code_balance_loss",
+    "CodeBalance",
 ]

@@ -31,6 +31,10 @@ GSB_PEER_HANDLE_BYTES = 64
 GSB_SORT_NOALLOC_MAX_PAIRS = 262144
 GSB_SORT_NOALLOC_SCRATCH_BYTES = 6 << 20
 GSB_DEVERR_PEER_TIMEOUT = 8
+GSB_DTYPE_F32 = 0
+GSB_DTYPE_BF16 = 1
+GSB_DTYPE_F16 = 2
+GSB_CODE_MAX_TOP = 32
 
 DEVERR_LOOKBACK_TIMEOUT = 1
 DEVERR_PAIR_OVERFLOW = 2
@@ -65,6 +69,14 @@ EXPORTED = (
     "gsb_radix_sort_pairs_noalloc",
     "gsb_sh_forward",
     "gsb_sh_backward",
+    "gsb_codebook_forward",
+    "gsb_codebook_backward_workspace_size",
+    "gsb_codebook_backward",
+    "gsb_code_log_probs_forward",
+    "gsb_code_log_probs_backward",
+    "gsb_code_balance_workspace_size",
+    "gsb_code_balance_forward",
+    "gsb_code_balance_backward",
     "gsb_peer_buffer_alloc",
     "gsb_peer_buffer_free",
     "gsb_peer_handle",
@@ -137,6 +149,15 @@ def load() -> C.CDLL:
         "gsb_radix_sort_pairs_noalloc": (C.c_int, [p, p, p, p, i64, C.c_int, C.c_int, p, p]),
         "gsb_sh_forward": (C.c_int, [i32, i32, i32, p, p, p, p, p]),
         "gsb_sh_backward": (C.c_int, [i32, i32, i32, p, p, p, p, p, p, p, p, p]),
+        "gsb_codebook_forward": (C.c_int, [i32, i32, i64, i32, i64, i32, p, i64, p, i32, p, f32, p, p, p]),
+        "gsb_codebook_backward_workspace_size": (sz, [i64, i32, i64, i32]),
+        "gsb_codebook_backward": (C.c_int, [i32, i32, i64, i32, i64, i32, p, i64, p, i32, p, f32, p, p, p, p, p, sz,
+                                            p]),
+        "gsb_code_log_probs_forward": (C.c_int, [i32, i64, i64, p, i64, p, i32, i32, p, p, p, p, p, p, p]),
+        "gsb_code_log_probs_backward": (C.c_int, [i32, i64, i64, p, i64, p, i32, i32, p, p, p, p, p, p, p]),
+        "gsb_code_balance_workspace_size": (sz, [i64, i64]),
+        "gsb_code_balance_forward": (C.c_int, [i32, i64, i64, i32, p, i64, p, i32, p, p, p, p, p, p, sz, p]),
+        "gsb_code_balance_backward": (C.c_int, [i32, i64, i64, p, i64, p, p, p, p, p, p]),
         "gsb_peer_buffer_alloc": (C.c_int, [sz, C.POINTER(p)]),
         "gsb_peer_buffer_free": (C.c_int, [p]),
         "gsb_peer_handle": (C.c_int, [p, p]),

@@ -271,8 +271,9 @@ _ops_ns = None
 
 def _ops():
     """torch.ops.gsplat_b200: rasterize_fwd, bin, render_fwd_eval,
-    render_fwd_train, render_bwd, project_fwd, project_bwd, sh_fwd, sh_bwd
-    (CUDA dispatch key only)."""
+    render_fwd_train, render_bwd, project_fwd, project_bwd, sh_fwd, sh_bwd,
+    codebook_fwd, codebook_bwd, code_log_probs_fwd, code_log_probs_bwd,
+    code_balance_fwd, code_balance_bwd (CUDA dispatch key only)."""
     global _ops_ns
     if _ops_ns is None:
         _host()

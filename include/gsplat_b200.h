@@ -252,6 +252,74 @@ int gsb_sh_backward(int32_t batch_size, int32_t gaussians, int32_t degree, const
                     const float* grad_colors, float* g_sh_coeffs, float* g_means3d,
                     float* g_camera_to_world, void* stream);
 
+/* ---- codebook attributes ---------------------------------------------------
+ * No reference counterpart: the reference keeps every attribute per splat. A
+ * compressed scene keeps a codebook of attribute rows (SH coefficients, say) and
+ * a code, or a few weighted codes, per splat; the codes are learned from
+ * assignment logits [rows, codebook_rows].
+ *
+ * Element types are GSB_DTYPE_*; sums are fp32 and rounded once. Codes are int32
+ * (code_bytes 4) or int64 (8), contiguous; a negative code is an empty slot. A
+ * code of codebook_rows or more is taken as empty too and raises
+ * GSB_DEVERR_BOUNDS in `status`, a status block in device memory or in mapped
+ * host memory. Strides are in elements, between rows; a row's values are
+ * contiguous. Outputs are contiguous. All results are the same from call to
+ * call: no sum depends on the order in which blocks run. */
+#define GSB_DTYPE_F32 0
+#define GSB_DTYPE_BF16 1
+#define GSB_DTYPE_F16 2
+#define GSB_CODE_MAX_TOP 32
+
+/* out[n, :] = scale * sum_j weights[n, j] * table[codes[n, j], :], j < bag.
+ * table [codebook_rows, dim] of table_dtype, codes [rows, bag], weights [rows, bag]
+ * (NULL: ones), out [rows, dim] of out_dtype. */
+int gsb_codebook_forward(int32_t table_dtype, int32_t out_dtype, int64_t rows, int32_t bag,
+                         int64_t codebook_rows, int32_t dim, const void* table, int64_t table_stride,
+                         const void* codes, int32_t code_bytes, const float* weights, float scale, void* out,
+                         uint32_t* status, void* stream);
+/* Its gradients: g_table [codebook_rows, dim] of table_dtype (every row written,
+ * zeros where a code is not used) and g_weights [rows, bag]; either may be NULL.
+ * grad_out [rows, dim] of out_dtype. The codes are sorted (rows * bag < 2^30);
+ * the workspace may be NULL without g_table. */
+size_t gsb_codebook_backward_workspace_size(int64_t rows, int32_t bag, int64_t codebook_rows, int32_t dim);
+int gsb_codebook_backward(int32_t table_dtype, int32_t out_dtype, int64_t rows, int32_t bag,
+                          int64_t codebook_rows, int32_t dim, const void* table, int64_t table_stride,
+                          const void* codes, int32_t code_bytes, const float* weights, float scale,
+                          const void* grad_out, void* g_table, float* g_weights, uint32_t* status,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* Per row of logits: log_probs = log softmax at the given code (0 for an empty
+ * one; codes and log_probs both given or both NULL), entropy = -sum p log p, and
+ * the top_k (0 .. GSB_CODE_MAX_TOP) largest log probabilities with their codes,
+ * ties to the lower code. A logit of -inf has probability 0; a row of nothing
+ * else has log probabilities -inf, entropy 0 and gradient 0. stats [rows, 4]
+ * (optional) is what the backward reads. */
+int gsb_code_log_probs_forward(int32_t dtype, int64_t rows, int64_t codebook_rows, const void* logits,
+                               int64_t logits_stride, const void* codes, int32_t code_bytes, int32_t top_k,
+                               float* log_probs, float* entropy, float* top_log_probs, int32_t* top_codes,
+                               float* stats, uint32_t* status, void* stream);
+/* Any incoming gradient may be NULL (zeros). g_logits [rows, codebook_rows] of dtype. */
+int gsb_code_log_probs_backward(int32_t dtype, int64_t rows, int64_t codebook_rows, const void* logits,
+                                int64_t logits_stride, const void* codes, int32_t code_bytes, int32_t top_k,
+                                const int32_t* top_codes, const float* stats, const float* g_log_probs,
+                                const float* g_entropy, const float* g_top_log_probs, void* g_logits,
+                                void* stream);
+
+/* Even use of the codes: with f_c the share of code c among all codes [rows, bag]
+ * and P_c the mean of softmax(logits)_c over the rows that have a code,
+ *   loss = codebook_rows * sum_c f_c P_c      (1 for even use; 0 without any code)
+ * and counts [codebook_rows] how often each code occurs. The gradient goes to the
+ * logits through P; counts are constants. stats [rows, 4] (optional) and coef [1]
+ * are what the backward reads. rows * bag < 2^31. */
+size_t gsb_code_balance_workspace_size(int64_t rows, int64_t codebook_rows);
+int gsb_code_balance_forward(int32_t dtype, int64_t rows, int64_t codebook_rows, int32_t bag,
+                             const void* logits, int64_t logits_stride, const void* codes, int32_t code_bytes,
+                             float* loss, int32_t* counts, float* stats, float* coef, uint32_t* status,
+                             void* workspace, size_t workspace_bytes, void* stream);
+int gsb_code_balance_backward(int32_t dtype, int64_t rows, int64_t codebook_rows, const void* logits,
+                              int64_t logits_stride, const int32_t* counts, const float* stats,
+                              const float* coef, const float* g_loss, void* g_logits, void* stream);
+
 /* ---- multi-GPU: gradient sum over NVLink peer memory -----------------------
  * No counterpart in the reference, which is single-device. Sums a float buffer
  * across the ranks of one node in place, replacing the NCCL all-reduce of the

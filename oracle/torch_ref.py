@@ -260,3 +260,50 @@ def harness_measure_accuracy(run_renderer, renderer: str, base_inputs, height: i
             worst.append(float(e.max().item()))
         result["grad_max_abs_error"] = max(worst) if worst else 0.0
     return result
+
+
+# ---------------------------------------------------------------------------
+# Codebook attributes, in 64 bits and differentiable by autograd. Negative codes
+# are empty slots.
+# ---------------------------------------------------------------------------
+def codebook_lookup_reference(codebook, codes, weights=None, scale: float = 1.0):
+    """scale * codebook[codes], summed over the last axis of codes with weights."""
+    zero = torch.zeros_like(codebook[:1])
+    rows = torch.cat([codebook, zero])[torch.where(codes < 0, codebook.shape[0], codes.long())]
+    if weights is not None:
+        w = weights.reshape(*weights.shape, *([1] * (codebook.ndim - 1)))
+        rows = (rows * w).sum(codes.ndim - 1)
+    return rows * scale
+
+
+def _code_log_softmax(logits):
+    """(log softmax, rows that hold more than -inf); the other rows count as even."""
+    some = (logits > float("-inf")).any(-1, keepdim=True)
+    return torch.log_softmax(torch.where(some, logits, torch.zeros_like(logits)), -1), some
+
+
+def code_log_probs_reference(logits, codes, top_k: int):
+    """(log_probs, entropy, top_log_probs, top_codes) of logits [..., C]."""
+    lp, some = _code_log_softmax(logits)
+    low = torch.full_like(lp, float("-inf"))
+    lp_out = torch.where(some, lp, low)
+    log_probs = None
+    if codes is not None:
+        log_probs = lp_out.gather(-1, codes.clamp(min=0).long()[..., None])[..., 0]
+        log_probs = torch.where(codes >= 0, log_probs, torch.zeros_like(log_probs))
+    entropy = -(lp.exp() * torch.where(torch.isinf(lp), torch.zeros_like(lp), lp)).sum(-1)
+    entropy = torch.where(some[..., 0], entropy, torch.zeros_like(entropy))
+    top_codes = torch.argsort(logits.detach(), dim=-1, descending=True, stable=True)[..., :top_k]
+    return log_probs, entropy, lp_out.gather(-1, top_codes), top_codes
+
+
+def code_balance_reference(logits, codes):
+    """(loss, counts) of logits [G, C] and codes [G, J]."""
+    C = logits.shape[-1]
+    lp, some = _code_log_softmax(logits)
+    chosen = codes[codes >= 0].long()
+    counts = torch.bincount(chosen, minlength=C)
+    valid = (codes >= 0).any(-1)
+    n = max(1, int(valid.sum()))
+    p = torch.where(some & valid[:, None], lp.exp(), torch.zeros_like(lp))
+    return C * (counts.to(lp.dtype) / max(1, chosen.numel()) * (p.sum(0) / n)).sum(), counts
