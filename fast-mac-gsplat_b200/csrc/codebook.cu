@@ -7,34 +7,90 @@
 // Sums are fp32, rounded once to the result's type. The table gradient sorts
 // the codes (stable radix sort), so each row is a sum in a fixed order: the
 // result does not depend on the timing of the blocks.
+#include <algorithm>
+#include <type_traits>
+
 #include "code_types.cuh"
 #include "radix_sort.cuh"
 
 namespace gsb {
 namespace {
 
-// One thread per output value.
-template <typename T, typename O>
+// V values of a row at once: V = 4 where rows, strides and addresses allow it.
+template <int V, typename T>
+struct Vec {
+  float v[V];
+  __device__ __forceinline__ void load(const T* __restrict__ p) {
+    if constexpr (V == 4 && sizeof(T) == 4) {
+      const float4 q = *reinterpret_cast<const float4*>(p);
+      v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+    } else if constexpr (V == 4) {
+      const uint2 q = *reinterpret_cast<const uint2*>(p);
+      const T* h = reinterpret_cast<const T*>(&q);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = to_f32(h[i]);
+    } else {
+      v[0] = to_f32(*p);
+    }
+  }
+};
+template <int V, typename T>
+__device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&v)[V]) {
+  if constexpr (V == 4 && sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  } else if constexpr (V == 4) {
+    uint2 q;
+    T* h = reinterpret_cast<T*>(&q);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = from_f32<T>(v[i]);
+    *reinterpret_cast<uint2*>(p) = q;
+  } else {
+    *p = from_f32<T>(v[0]);
+  }
+}
+
+// One thread per V values of the result and kLookupItems such pieces, a block's
+// width apart: stores of a warp are contiguous whatever the row's length, and the
+// loads of the pieces (code, then row) overlap. Bound by the stores: the table
+// and the codes of neighbouring threads come from L2 and L1.
+constexpr int kLookupItems = 4;
+template <typename T, typename O, int V>
 __global__ void __launch_bounds__(256)
-    k_lookup(int64_t total, int bag, int64_t C, int dim, const T* __restrict__ table, int64_t stride, Codes codes,
-             const float* __restrict__ weights, float scale, O* __restrict__ out, uint32_t* status) {
+    k_lookup(int64_t pieces, int bag, int64_t C, int nvec, FastDiv div_nvec, const T* __restrict__ table,
+             int64_t stride, Codes codes, const float* __restrict__ weights, float scale, O* __restrict__ out,
+             uint32_t* status) {
   pdl_wait();
   pdl_trigger();
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= total) return;
-  const int64_t n = i / dim;
-  const int d = (int)(i - n * dim);
-  float acc = 0.0f;
-  for (int j = 0; j < bag; ++j) {
-    const int64_t c = codes.at(n * bag + j);
-    if (c < 0) continue;
-    if (c >= C) {
-      bad_code(status, kSiteCode);
-      continue;
+  const int64_t tile = (int64_t)blockIdx.x * (256 * kLookupItems);
+  const int64_t row0 = tile / nvec;
+  const int off0 = (int)(tile - row0 * nvec);
+#pragma unroll
+  for (int k = 0; k < kLookupItems; ++k) {
+    const int local = off0 + k * 256 + (int)threadIdx.x;
+    if (tile + (local - off0) >= pieces) break;
+    const int r = fast_div(local, div_nvec);
+    const int64_t n = row0 + r;
+    const int d = (local - r * nvec) * V;
+    float acc[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+    for (int j = 0; j < bag; ++j) {
+      const int64_t c = codes.at(n * bag + j);
+      if (c < 0) continue;
+      if (c >= C) {
+        bad_code(status, kSiteCode);
+        continue;
+      }
+      const float w = weights ? weights[n * bag + j] : 1.0f;
+      Vec<V, T> t;
+      t.load(table + c * stride + d);
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] = fmaf(w, t.v[i], acc[i]);
     }
-    acc = fmaf(weights ? weights[n * bag + j] : 1.0f, to_f32(table[c * stride + d]), acc);
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] *= scale;
+    store_vec<V>(out + (tile + (local - off0)) * V, acc);
   }
-  out[i] = from_f32<O>(acc * scale);
 }
 
 // Sort keys: the code, or C for an empty slot (sorted behind every code).
@@ -51,34 +107,227 @@ __global__ void __launch_bounds__(256)
   vals[i] = (uint32_t)i;
 }
 
-// One warp per codebook row: its entries are found by bisection.
-template <typename T, typename O>
+// Sums of the sorted entries, run by run (a run: the entries of one code).
+//
+// A group of GL lanes adds up kRunEntries consecutive entries, each lane R
+// pieces of V columns; a block of 256 threads takes 256 / GL such stretches. A
+// run inside a stretch is written at once. A run that crosses stretches leaves
+// its parts in shared memory, where the group it starts in adds them up, and one
+// that crosses blocks leaves at most two parts per block (head: of a run begun
+// in an earlier block; tail: of one that goes on) for k_run_parts. So every row
+// is a sum in one order, however uneven the codes are, and a code that all
+// entries share costs no more than an even use.
+//
+// Bound by the gather of g: rows in code order, one load of the whole row per
+// entry. With WGRAD the same loads give g_w (GL lanes share a dot product); that
+// takes the row in one tile of columns.
+constexpr int kRunEntries = 16;
+constexpr int kRunBlockEntries = 2048;  // at most, per block
+template <int GL>
+constexpr int run_entries() { return kRunBlockEntries / (256 / GL) < kRunEntries ? kRunBlockEntries / (256 / GL) : kRunEntries; }
+template <int GL>
+constexpr int run_block_entries() { return run_entries<GL>() * (256 / GL); }
+
+template <typename T, typename O, int V, int GL, int R, bool WGRAD>
 __global__ void __launch_bounds__(256)
-    k_table_grad(int64_t n, int bag, int64_t C, int dim, const uint32_t* __restrict__ keys,
-                 const uint32_t* __restrict__ vals, const float* __restrict__ weights, float scale,
-                 const O* __restrict__ g, T* __restrict__ g_table) {
+    k_run_sums(int n, int bag, FastDiv div_bag, int C, int dim, const uint32_t* __restrict__ keys,
+               const uint32_t* __restrict__ vals, const float* __restrict__ weights, float scale,
+               const O* __restrict__ g, const T* __restrict__ table, int64_t stride, T* __restrict__ g_table,
+               float* __restrict__ g_weights, float* __restrict__ parts) {
   pdl_wait();
   pdl_trigger();
-  const int64_t c = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (c >= C) return;
-  auto first = [&](uint32_t key) {
-    int64_t lo = 0, hi = n;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (keys[mid] < key) lo = mid + 1;
-      else hi = mid;
-    }
-    return lo;
+  constexpr int NG = 256 / GL, E = run_entries<GL>(), L = run_block_entries<GL>(), W = GL * V * R;
+  constexpr int U = WGRAD ? 2 : 4;  // entries whose loads are in flight together
+  __shared__ uint32_t s_key[L + 2];  // the entries' keys, with the neighbours' on either side
+  __shared__ uint32_t s_val[L];
+  __shared__ __align__(16) float s_part[2][NG][W];
+  const int tid = threadIdx.x, lane = tid % GL, grp = tid / GL;
+  const int64_t b0 = (int64_t)blockIdx.x * L;
+  const int cnt = (int)min((int64_t)L, n - b0);
+  const uint32_t kNone = 0xffffffffu;  // no entry: differs from every key
+  for (int i = tid; i < L + 2; i += 256) {
+    const int64_t k = b0 + i - 1;
+    s_key[i] = k >= 0 && k < n ? keys[k] : kNone;
+    if (i >= 1 && i <= L) s_val[i - 1] = i <= cnt ? vals[k] : 0u;
+  }
+  __syncthreads();
+  const int col0 = (int)blockIdx.y * W + lane * V;
+  const int s = grp * E, e = min(s + E, cnt);
+  float acc[R][V];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[r][i] = 0.0f;
+  bool head = s < e && s_key[s] == s_key[s + 1];  // the run in hand began before this stretch
+  auto put = [&](float* to) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < V; ++i) to[(r * GL + lane) * V + i] = acc[r][i];
   };
-  const int64_t lo = first((uint32_t)c), hi = first((uint32_t)c + 1u);
-  for (int d = lane; d < dim; d += 32) {
-    float acc = 0.0f;
-    for (int64_t k = lo; k < hi; ++k) {
-      const uint32_t v = vals[k];
-      acc = fmaf(weights ? weights[v] : 1.0f, to_f32(g[(int64_t)(v / (uint32_t)bag) * dim + d]), acc);
+  auto write_row = [&](uint32_t key) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int d = col0 + r * GL * V;
+      if (d < dim) {
+        float v[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = acc[r][i] * scale;
+        store_vec<V>(g_table + (int64_t)key * dim + d, v);
+      }
     }
-    g_table[c * dim + d] = from_f32<T>(acc * scale);
+  };
+  // As many turns for every group of a warp: the dot products exchange lanes.
+  for (int k0 = s; k0 < s + E; k0 += U) {
+    float w[U];
+    Vec<V, O> x[U][R];
+    Vec<V, T> t[WGRAD ? U : 1][R];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u;
+      const uint32_t key = k < e ? s_key[k + 1] : (uint32_t)C;
+      const uint32_t v = k < e ? s_val[k] : 0u;
+      const bool on = key < (uint32_t)C;
+      w[u] = on ? (weights ? weights[v] : 1.0f) : 0.0f;
+      const int64_t row = fast_div((int)v, div_bag);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int d = col0 + r * GL * V;
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[u][r].v[i] = 0.0f;
+        if (on && d < dim) x[u][r].load(g + row * dim + d);
+        if constexpr (WGRAD) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) t[u][r].v[i] = 0.0f;
+          if (on && d < dim) t[u][r].load(table + (int64_t)key * stride + d);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u;
+      if constexpr (WGRAD) {
+        float dot = 0.0f;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int i = 0; i < V; ++i) dot = fmaf(x[u][r].v[i], t[u][r].v[i], dot);
+#pragma unroll
+        for (int o = GL / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(kFullMask, dot, o, GL);
+        if (lane == 0 && k < e) g_weights[s_val[k]] = dot * scale;
+      }
+      if (k < e) {
+        const uint32_t key = s_key[k + 1];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[r][i] = fmaf(w[u], x[u][r].v[i], acc[r][i]);
+        const bool ends = s_key[k + 2] != key;
+        if ((ends || k == e - 1) && key < (uint32_t)C) {
+          if (head) put(s_part[0][grp]);
+          else if (ends) write_row(key);
+          else put(s_part[1][grp]);
+        }
+        if (ends) {
+          head = false;
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[r][i] = 0.0f;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (s >= e) return;
+  // The runs that cross stretches: the group a run starts in takes its tail and
+  // the heads after it; group 0 also takes a run from before the block.
+  auto chain = [&](int from) {  // adds the heads of stretches from, from + 1, ... ; true if the run goes on behind the block
+    for (int j = from; j < NG; ++j) {
+      const float* h = s_part[0][j];
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[r][i] += h[(r * GL + lane) * V + i];
+      const int je = min((j + 1) * E, cnt);
+      // One run from the stretch's first entry to its last, and on.
+      if (s_key[j * E + 1] != s_key[je] || s_key[je + 1] != s_key[je]) return false;
+      if (je == cnt) return true;
+    }
+    return true;
+  };
+  auto put_block = [&](int which) {
+    float* to = parts + ((int64_t)blockIdx.x * 2 + which) * dim;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int d = col0 + r * GL * V;
+      if (d < dim)
+#pragma unroll
+        for (int i = 0; i < V; ++i) to[d + i] = acc[r][i];
+    }
+  };
+  auto clear = [&]() {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[r][i] = 0.0f;
+  };
+  if (grp == 0 && s_key[0] == s_key[1] && s_key[1] < (uint32_t)C) {
+    clear();
+    chain(0);
+    put_block(0);
+  }
+  const uint32_t last = s_key[e];
+  const bool goes_on = s_key[e + 1] == last && last < (uint32_t)C;
+  const bool began_here = s_key[s] != s_key[s + 1] || s_key[s + 1] != last;  // the last run starts in this stretch
+  if (goes_on && began_here) {
+    const float* h = s_part[1][grp];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[r][i] = h[(r * GL + lane) * V + i];
+    if (e == cnt || chain(grp + 1)) put_block(1);
+    else write_row(last);
+  }
+}
+
+// The runs that cross blocks of k_run_sums: the block a run starts in adds its
+// tail and the heads of the blocks after it, 256 / columns of them at a time.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    k_run_parts(int n, int C, int dim, int block_entries, const uint32_t* __restrict__ keys, float scale,
+                const float* __restrict__ parts, T* __restrict__ g_table) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ float s_sum[256];
+  const int64_t b0 = (int64_t)blockIdx.x * block_entries, end = b0 + block_entries;
+  if (end >= n) return;
+  const uint32_t key = keys[end - 1];
+  if (key >= (uint32_t)C || keys[end] != key || (b0 > 0 && keys[b0 - 1] == key)) return;
+  int64_t lo = end, hi = n;  // first entry behind the run
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (keys[mid] <= key) lo = mid + 1;
+    else hi = mid;
+  }
+  const int64_t heads = (lo - 1) / block_entries - blockIdx.x;
+  const int cols = min(dim, 256), ways = 256 / cols;
+  const int way = threadIdx.x / cols, col = threadIdx.x - way * cols;
+  for (int d0 = 0; d0 < dim; d0 += cols) {
+    const int d = d0 + col;
+    float acc = 0.0f;
+    if (way < ways && d < dim) {
+      const float* p = parts + (int64_t)blockIdx.x * 2 * dim + d;
+      if (way == 0) acc = p[dim];
+      for (int64_t h = 1 + way; h <= heads; h += ways) acc += p[h * 2 * dim];
+    }
+    s_sum[threadIdx.x] = acc;
+    __syncthreads();
+    if (way == 0 && d < dim) {
+      for (int i = 1; i < ways; ++i) acc += s_sum[i * cols + col];
+      g_table[(int64_t)key * dim + d] = from_f32<T>(acc * scale);
+    }
+    __syncthreads();
   }
 }
 
@@ -105,24 +354,82 @@ __global__ void __launch_bounds__(256)
   if (lane == 0) g_weights[i] = acc * scale;
 }
 
+// How the columns of a row are dealt out: V values a piece, GL lanes a row, R = 2
+// or 3 pieces a lane, whichever leaves fewer lanes idle; more columns take more tiles.
+struct RunShape {
+  int V, GL, R;
+  int block_entries() const {
+    const int ng = 256 / GL;
+    return ng * std::min(kRunEntries, kRunBlockEntries / ng);
+  }
+  int tiles(int dim) const { return (dim + V * GL * R - 1) / (V * GL * R); }
+};
+RunShape run_shape(int dim, int V) {
+  const int nvec = (dim + V - 1) / V;
+  RunShape best{V, 32, 3};
+  int waste = 1 << 30;
+  for (int R = 3; R >= 2; --R) {
+    int GL = 1;
+    while (GL < 32 && GL * R < nvec) GL *= 2;
+    if (GL * R < nvec) continue;
+    if (GL * R - nvec < waste) {
+      waste = GL * R - nvec;
+      best = RunShape{V, GL, R};
+    }
+  }
+  return best;
+}
+
 struct BackwardScratch {
   uint32_t *keys = nullptr, *vals = nullptr, *keys_s = nullptr, *vals_s = nullptr;
+  float* parts = nullptr;
 };
-BackwardScratch carve(Carver& ws, int64_t slots) {
+BackwardScratch carve(Carver& ws, int64_t slots, int dim) {
   BackwardScratch b;
   b.keys = ws.take<uint32_t>((size_t)slots);
   b.vals = ws.take<uint32_t>((size_t)slots);
   b.keys_s = ws.take<uint32_t>((size_t)slots);
   b.vals_s = ws.take<uint32_t>((size_t)slots);
+  const int64_t least = std::min(run_shape(dim, 1).block_entries(), run_shape(dim, 4).block_entries());
+  b.parts = ws.take<float>((size_t)((slots + least - 1) / least) * 2 * (size_t)dim);
   return b;
+}
+
+inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// Calls fn(T{}, O{}) for the element types of table and result.
+template <typename Fn>
+void with_dtypes(int32_t table_dtype, int32_t out_dtype, Fn&& fn) {
+  with_dtype(table_dtype, [&](auto t) {
+    if (out_dtype == GSB_DTYPE_F32) fn(t, float{});
+    else fn(t, t);
+  });
+}
+
+// Calls fn(integral constants GL, R).
+template <typename Fn>
+void with_shape(const RunShape& s, Fn&& fn) {
+  auto lanes = [&](auto r) {
+    switch (s.GL) {
+      case 1: fn(std::integral_constant<int, 1>{}, r); break;
+      case 2: fn(std::integral_constant<int, 2>{}, r); break;
+      case 4: fn(std::integral_constant<int, 4>{}, r); break;
+      case 8: fn(std::integral_constant<int, 8>{}, r); break;
+      case 16: fn(std::integral_constant<int, 16>{}, r); break;
+      default: fn(std::integral_constant<int, 32>{}, r); break;
+    }
+  };
+  if (s.R == 2) lanes(std::integral_constant<int, 2>{});
+  else lanes(std::integral_constant<int, 3>{});
 }
 
 // Sizes common to both directions; the blocks of a launch have to fit the grid.
 int check_sizes(int32_t table_dtype, int32_t out_dtype, int64_t rows, int32_t bag, int64_t codebook_rows, int32_t dim,
                 int64_t stride, int32_t code_bytes) {
-  if (!dtype_ok(table_dtype) || !dtype_ok(out_dtype)) return GSB_ERR_UNSUPPORTED;
+  if (!dtype_ok(table_dtype) || (out_dtype != table_dtype && out_dtype != GSB_DTYPE_F32)) return GSB_ERR_UNSUPPORTED;
   if (rows < 0 || bag <= 0 || codebook_rows <= 0 || dim <= 0 || stride < 0 || (code_bytes != 4 && code_bytes != 8))
     return GSB_ERR_INVALID_ARGUMENT;
+  // Column tiles of the gradient are at least 96 wide and fit the grid's 65,535.
   if (codebook_rows >= (int64_t(1) << 31) - 1 || rows > kSortMaxN / bag || dim > (1 << 20)) return GSB_ERR_CAPACITY;
   return GSB_OK;
 }
@@ -140,16 +447,18 @@ extern "C" int gsb_codebook_forward(int32_t table_dtype, int32_t out_dtype, int6
   if (rc != GSB_OK) return rc;
   if (rows == 0) return GSB_OK;
   if (!table || !codes || !out || !status) return GSB_ERR_INVALID_ARGUMENT;
-  const int64_t total = rows * dim;
-  if ((total + 255) / 256 >= (int64_t(1) << 31)) return GSB_ERR_CAPACITY;
   const Codes cd{codes, code_bytes == 8};
-  with_dtype(table_dtype, [&](auto t) {
-    with_dtype(out_dtype, [&](auto o) {
+  const int so = dtype_bytes(out_dtype), st = dtype_bytes(table_dtype);
+  const int V = dim % 4 == 0 && table_stride % 4 == 0 && aligned_to(table, 4 * st) && aligned_to(out, 4 * so) ? 4 : 1;
+  const int64_t pieces = rows * (dim / V);
+  const int64_t blocks = (pieces + 256 * kLookupItems - 1) / (256 * kLookupItems);
+  if (blocks >= (int64_t(1) << 31)) return GSB_ERR_CAPACITY;
+  with_dtypes(table_dtype, out_dtype, [&](auto t, auto o) {
       using T = decltype(t);
       using O = decltype(o);
-      launch_pdl(k_lookup<T, O>, grid1d(total, 256), 256, 0, static_cast<cudaStream_t>(stream), total, bag,
-                 codebook_rows, dim, (const T*)table, table_stride, cd, weights, scale, (O*)out, status);
-    });
+      launch_pdl(V == 4 ? k_lookup<T, O, 4> : k_lookup<T, O, 1>, (unsigned)blocks, 256, 0,
+                 static_cast<cudaStream_t>(stream), pieces, bag, codebook_rows, dim / V,
+                 make_fast_div((uint32_t)(dim / V)), (const T*)table, table_stride, cd, weights, scale, (O*)out, status);
   });
   note_launches(1);
   return cuda_status(cudaGetLastError());
@@ -159,7 +468,7 @@ extern "C" size_t gsb_codebook_backward_workspace_size(int64_t rows, int32_t bag
   if (check_sizes(GSB_DTYPE_F32, GSB_DTYPE_F32, rows, bag, codebook_rows, dim, 0, 4) != GSB_OK) return 0;
   const int64_t slots = rows * bag;
   Carver c(nullptr);
-  carve(c, slots);
+  carve(c, slots, dim);
   radix_sort_pairs(c, (const uint32_t*)nullptr, nullptr, nullptr, nullptr, slots, 0, bits_for(codebook_rows), nullptr,
                    0, false);
   return c.off + 256;
@@ -186,29 +495,43 @@ extern "C" int gsb_codebook_backward(int32_t table_dtype, int32_t out_dtype, int
     if (!workspace || workspace_bytes < gsb_codebook_backward_workspace_size(rows, bag, codebook_rows, dim))
       return GSB_ERR_WORKSPACE;
     Carver ws(workspace);
-    const BackwardScratch b = carve(ws, slots);
+    const BackwardScratch b = carve(ws, slots, dim);
+    if (cudaMemsetAsync(g_table, 0, (size_t)codebook_rows * dim * dtype_bytes(table_dtype), s) != cudaSuccess)
+      return GSB_ERR_CUDA;  // the rows that no code names
     launch_pdl(k_code_keys, grid1d(slots, 256), 256, 0, s, slots, codebook_rows, cd, b.keys, b.vals, status);
     e = radix_sort_pairs(ws, b.keys, b.vals, b.keys_s, b.vals_s, slots, 0, bits_for(codebook_rows), status, s, false);
     if (e != cudaSuccess) return GSB_ERR_CUDA;
-    with_dtype(table_dtype, [&](auto t) {
-      with_dtype(out_dtype, [&](auto o) {
+    const int so = dtype_bytes(out_dtype), st = dtype_bytes(table_dtype);
+    const bool vec = dim % 4 == 0 && aligned_to(grad_out, 4 * so) && aligned_to(g_table, 4 * st) &&
+                     (!g_weights || (table_stride % 4 == 0 && aligned_to(table, 4 * st)));
+    const RunShape shape = run_shape(dim, vec ? 4 : 1);
+    const int block_entries = shape.block_entries();
+    const dim3 grid((unsigned)((slots + block_entries - 1) / block_entries), (unsigned)shape.tiles(dim));
+    const bool fused = g_weights && shape.tiles(dim) == 1;
+    with_dtypes(table_dtype, out_dtype, [&](auto t, auto o) {
         using T = decltype(t);
         using O = decltype(o);
-        launch_pdl(k_table_grad<T, O>, grid1d(codebook_rows * 32, 256), 256, 0, s, slots, bag, codebook_rows, dim,
-                   (const uint32_t*)b.keys_s, (const uint32_t*)b.vals_s, weights, scale, (const O*)grad_out,
-                   (T*)g_table);
-      });
+        with_shape(shape, [&](auto gl, auto r) {
+          constexpr int GL = decltype(gl)::value, R = decltype(r)::value;
+          auto kernel = vec ? (fused ? k_run_sums<T, O, 4, GL, R, true> : k_run_sums<T, O, 4, GL, R, false>)
+                            : (fused ? k_run_sums<T, O, 1, GL, R, true> : k_run_sums<T, O, 1, GL, R, false>);
+          launch_pdl(kernel, grid, 256, 0, s, (int)slots, bag, make_fast_div((uint32_t)bag), (int)codebook_rows, dim,
+                     (const uint32_t*)b.keys_s, (const uint32_t*)b.vals_s, weights, scale, (const O*)grad_out,
+                     (const T*)table, table_stride, (T*)g_table, g_weights, b.parts);
+        });
+        if (grid.x > 1)
+          launch_pdl(k_run_parts<T>, grid.x - 1, 256, 0, s, (int)slots, (int)codebook_rows, dim, block_entries,
+                     (const uint32_t*)b.keys_s, scale, (const float*)b.parts, (T*)g_table);
     });
-    note_launches(2);
+    note_launches(grid.x > 1 ? 3 : 2);
+    if (fused) g_weights = nullptr;  // done
   }
   if (g_weights) {
-    with_dtype(table_dtype, [&](auto t) {
-      with_dtype(out_dtype, [&](auto o) {
+    with_dtypes(table_dtype, out_dtype, [&](auto t, auto o) {
         using T = decltype(t);
         using O = decltype(o);
         launch_pdl(k_weight_grad<T, O>, grid1d(slots * 32, 256), 256, 0, s, slots, bag, codebook_rows, dim,
                    (const T*)table, table_stride, cd, scale, (const O*)grad_out, g_weights, status);
-      });
     });
     note_launches(1);
   }

@@ -817,6 +817,8 @@ Tensor op_codebook_fwd(const Tensor& codebook, const Tensor& codes, const std::o
                        at::ScalarType out_dtype) {
   const int32_t dt = code_dtype(codebook, "codebook");
   const c10::cuda::CUDAGuard guard(codebook.device());
+  if (out_dtype != codebook.scalar_type() && out_dtype != at::kFloat)
+    value_error("gsplat_b200: out_dtype must be the codebook's or float32");
   const LookupShape shape = lookup_shape(codebook, codes, weights);
   const Tensor t = table_rows(codebook), c = code_tensor(codes, codebook);
   const Tensor w = weights.has_value() && weights->defined() ? weights->contiguous() : Tensor();
@@ -838,6 +840,8 @@ std::tuple<Tensor, Tensor> op_codebook_bwd(const Tensor& grad_out, const Tensor&
   const c10::cuda::CUDAGuard guard(codebook.device());
   const LookupShape shape = lookup_shape(codebook, codes, weights);
   if (grad_out.sizes() != at::IntArrayRef(shape.out)) value_error("gsplat_b200: grad_out has another shape");
+  if (grad_out.scalar_type() != codebook.scalar_type() && grad_out.scalar_type() != at::kFloat)
+    value_error("gsplat_b200: grad_out must be of the codebook's type or float32");
   const Tensor t = table_rows(codebook), c = code_tensor(codes, codebook), g = grad_out.contiguous();
   const Tensor w = weights.has_value() && weights->defined() ? weights->contiguous() : Tensor();
   uint32_t* status = codebook_status(t);

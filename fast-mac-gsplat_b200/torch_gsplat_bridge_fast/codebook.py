@@ -118,7 +118,7 @@ def codebook_lookup(codebook: Tensor, codes: Tensor, weights: Optional[Tensor] =
     """scale * codebook[codes]: codebook [C, ...], codes of any shape -> [*codes.shape, ...].
     With float32 weights of the shape [..., J] of the codes, the J rows of the last
     axis are added up with them -> [...] + codebook.shape[1:]. Empty slots add
-    nothing; a result without any is zero. `out_dtype` defaults to the codebook's.
+    nothing; a result without any is zero. `out_dtype` is the codebook's or float32.
 
     Differentiable in codebook and weights. The codebook's rows may be strided
     (`sh[:, :9]`); its gradient sums the uses of a row in a fixed order."""
@@ -133,8 +133,8 @@ def codebook_lookup(codebook: Tensor, codes: Tensor, weights: Optional[Tensor] =
             raise ValueError("weights and codebook must be on the same CUDA device")
     if out_dtype is None:
         out_dtype = codebook.dtype
-    elif out_dtype not in _FLOATS:
-        raise ValueError("out_dtype must be float32, bfloat16 or float16")
+    elif out_dtype != codebook.dtype and out_dtype != torch.float32:
+        raise ValueError("out_dtype must be the codebook's or float32")
     _check("codebook", codebook, codes)
     if torch.is_grad_enabled() and (codebook.requires_grad or (weights is not None and weights.requires_grad)):
         return _Lookup.apply(codebook, codes, weights, float(scale), out_dtype)

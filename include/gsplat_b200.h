@@ -272,7 +272,7 @@ int gsb_sh_backward(int32_t batch_size, int32_t gaussians, int32_t degree, const
 
 /* out[n, :] = scale * sum_j weights[n, j] * table[codes[n, j], :], j < bag.
  * table [codebook_rows, dim] of table_dtype, codes [rows, bag], weights [rows, bag]
- * (NULL: ones), out [rows, dim] of out_dtype. */
+ * (NULL: ones), out [rows, dim] of out_dtype: table_dtype or GSB_DTYPE_F32. */
 int gsb_codebook_forward(int32_t table_dtype, int32_t out_dtype, int64_t rows, int32_t bag,
                          int64_t codebook_rows, int32_t dim, const void* table, int64_t table_stride,
                          const void* codes, int32_t code_bytes, const float* weights, float scale, void* out,

@@ -93,7 +93,7 @@ def test_c_entries_refuse_before_any_launch():
     one = 256  # a pointer that is never followed: each call is refused first
     fwd = lambda td=0, od=0, rows=4, bag=1, c=8, dim=3, table=one, stride=3, codes=one, cb=4, out=one, st=one: \
         L.gsb_codebook_forward(td, od, rows, bag, c, dim, table, stride, codes, cb, None, 1.0, out, st, None)
-    assert fwd(td=3) == 2 and fwd(od=-1) == 2
+    assert fwd(td=3) == 2 and fwd(od=-1) == 2 and fwd(od=1) == 2 and fwd(td=1, od=2) == 2
     for bad in (dict(rows=-1), dict(bag=0), dict(c=0), dict(dim=0), dict(cb=2), dict(table=None), dict(codes=None),
                 dict(out=None), dict(st=None), dict(stride=-1)):
         assert fwd(**bad) == 1, bad
@@ -217,10 +217,10 @@ def test_lookup_matches_reference(dtype, rows, C, row, bag, wide):
 @pytest.mark.gpu
 def test_lookup_out_types_mix():
     table, codes, w = _lookup_case(515, 40, (9, 3), 2, torch.float32, seed=8)
-    for out in DTYPES:
-        _check_lookup(table, codes, w, 1.0, out)
-    table, codes, w = _lookup_case(515, 40, (9, 3), 0, torch.bfloat16, seed=9)
-    _check_lookup(table, codes, w, 1.0, torch.float16)
+    _check_lookup(table, codes, w, 1.0, torch.float32)
+    for dtype, other in ((torch.float32, torch.bfloat16), (torch.bfloat16, torch.float16)):
+        with pytest.raises(ValueError, match="out_dtype"):
+            tgb.codebook_lookup(table.to(dtype), codes, w, out_dtype=other)
 
 
 @pytest.mark.gpu
