@@ -895,10 +895,14 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> op_code_log_probs_fwd(const T
   uint32_t* status = codebook_status(z);
   Tensor ent = empty(lead, at::kFloat, dev), tl = empty(topped, at::kFloat, dev), tc = empty(topped, at::kInt, dev);
   if (save_state) stats = empty({z.size(0), 4}, at::kFloat, dev);
+  const size_t ws_bytes = gsb_code_log_probs_workspace_size(z.size(0), z.size(1), static_cast<int32_t>(top_k));
+  Tensor ws;
+  if (ws_bytes > 0) ws = empty({static_cast<int64_t>(ws_bytes)}, at::kByte, dev);
   check(gsb_code_log_probs_forward(dt, z.size(0), z.size(1), z.data_ptr(), z.stride(0),
                                    c.defined() ? c.data_ptr() : nullptr, c.defined() ? code_bytes(c) : 4,
                                    static_cast<int32_t>(top_k), ptr<float>(lp), ptr<float>(ent), ptr<float>(tl),
-                                   ptr<int32_t>(tc), ptr<float>(stats), status, stream_of(z)),
+                                   ptr<int32_t>(tc), ptr<float>(stats), status, ws.defined() ? ws.data_ptr() : nullptr,
+                                   ws_bytes, stream_of(z)),
         "gsb_code_log_probs_forward");
   codebook_done(z);
   return {lp, ent, tl, tc, stats};
@@ -926,13 +930,13 @@ Tensor op_code_log_probs_bwd(const std::optional<Tensor>& g_log_probs, const std
   Tensor dz = empty(logits.sizes(), logits.scalar_type(), z.device());
   check(gsb_code_log_probs_backward(dt, rows, z.size(1), z.data_ptr(), z.stride(0),
                                     c.defined() ? c.data_ptr() : nullptr, c.defined() ? code_bytes(c) : 4,
-                                    static_cast<int32_t>(top_k), ptr<int32_t>(tc), ptr<float>(stats.contiguous()),
+                                    static_cast<int32_t>(top_k), ptr<int32_t>(tc), ptr<float>(aligned(stats, 16)),
                                     ptr<float>(gl), ptr<float>(gh), ptr<float>(gt), dz.data_ptr(), stream_of(z)),
         "gsb_code_log_probs_backward");
   return dz;
 }
 
-// -> loss [], counts [C], stats [rows,4] (undefined unless save_state), coef [1].
+// -> loss [], counts [C], stats [rows,4] (undefined unless save_state), state.
 std::tuple<Tensor, Tensor, Tensor, Tensor> op_code_balance_fwd(const Tensor& logits, const Tensor& codes,
                                                                bool save_state) {
   const int32_t dt = code_dtype(logits, "logits");
@@ -948,32 +952,32 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> op_code_balance_fwd(const Tensor& log
   }
   if (given != lead || bag < 1) value_error("gsplat_b200: codes must have the shape [...] or [...,J] of logits");
   uint32_t* status = codebook_status(z);
-  Tensor loss = empty({}, at::kFloat, dev), counts = empty({C}, at::kInt, dev), coef = empty({1}, at::kFloat, dev);
+  Tensor loss = empty({}, at::kFloat, dev), counts = empty({C}, at::kInt, dev);
+  Tensor state = empty({gsb_code_balance_state_floats(C)}, at::kFloat, dev);
   Tensor stats;
   if (save_state) stats = empty({rows, 4}, at::kFloat, dev);
   const size_t ws_bytes = gsb_code_balance_workspace_size(rows, C);
   Tensor ws = empty({static_cast<int64_t>(std::max<size_t>(ws_bytes, 1))}, at::kByte, dev);
   check(gsb_code_balance_forward(dt, rows, C, static_cast<int32_t>(bag), z.data_ptr(), z.stride(0), c.data_ptr(),
                                  code_bytes(c), ptr<float>(loss), ptr<int32_t>(counts), ptr<float>(stats),
-                                 ptr<float>(coef), status, ws.data_ptr(), ws_bytes, stream_of(z)),
+                                 ptr<float>(state), status, ws.data_ptr(), ws_bytes, stream_of(z)),
         "gsb_code_balance_forward");
   codebook_done(z);
-  return {loss, counts, stats, coef};
+  return {loss, counts, stats, state};
 }
 
-Tensor op_code_balance_bwd(const Tensor& g_loss, const Tensor& logits, const Tensor& counts, const Tensor& stats,
-                           const Tensor& coef) {
+Tensor op_code_balance_bwd(const Tensor& g_loss, const Tensor& logits, const Tensor& stats, const Tensor& state) {
   const int32_t dt = code_dtype(logits, "logits");
   const c10::cuda::CUDAGuard guard(logits.device());
   const Tensor z = logit_rows(logits), g = g_loss.to(at::kFloat).contiguous();
   check_same_device(g, logits, "g_loss");
-  if (g.numel() != 1 || coef.numel() != 1 || counts.numel() != z.size(1) || counts.scalar_type() != at::kInt ||
-      stats.numel() != z.size(0) * 4 || stats.scalar_type() != at::kFloat)
+  if (g.numel() != 1 || state.numel() != gsb_code_balance_state_floats(z.size(1)) ||
+      state.scalar_type() != at::kFloat || stats.numel() != z.size(0) * 4 || stats.scalar_type() != at::kFloat)
     value_error("gsplat_b200: the gradient does not match the forward's outputs");
   Tensor dz = empty(logits.sizes(), logits.scalar_type(), z.device());
   check(gsb_code_balance_backward(dt, z.size(0), z.size(1), z.data_ptr(), z.stride(0),
-                                  ptr<int32_t>(counts.contiguous()), ptr<float>(stats.contiguous()), ptr<float>(coef),
-                                  ptr<float>(g), dz.data_ptr(), stream_of(z)),
+                                  ptr<float>(aligned(stats, 16)), ptr<float>(aligned(state, 16)), ptr<float>(g),
+                                  dz.data_ptr(), stream_of(z)),
         "gsb_code_balance_backward");
   return dz;
 }
@@ -1037,8 +1041,8 @@ TORCH_LIBRARY(gsplat_b200, m) {
   m.def("code_log_probs_bwd(Tensor? g_log_probs, Tensor? g_entropy, Tensor? g_top_log_probs, Tensor logits, "
         "Tensor? codes, Tensor top_codes, Tensor stats) -> Tensor");
   m.def("code_balance_fwd(Tensor logits, Tensor codes, bool save_state) -> (Tensor loss, Tensor counts, Tensor stats, "
-        "Tensor coef)");
-  m.def("code_balance_bwd(Tensor g_loss, Tensor logits, Tensor counts, Tensor stats, Tensor coef) -> Tensor");
+        "Tensor state)");
+  m.def("code_balance_bwd(Tensor g_loss, Tensor logits, Tensor stats, Tensor state) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(gsplat_b200, CUDA, m) {

@@ -72,8 +72,10 @@ EXPORTED = (
     "gsb_codebook_forward",
     "gsb_codebook_backward_workspace_size",
     "gsb_codebook_backward",
+    "gsb_code_log_probs_workspace_size",
     "gsb_code_log_probs_forward",
     "gsb_code_log_probs_backward",
+    "gsb_code_balance_state_floats",
     "gsb_code_balance_workspace_size",
     "gsb_code_balance_forward",
     "gsb_code_balance_backward",
@@ -153,11 +155,13 @@ def load() -> C.CDLL:
         "gsb_codebook_backward_workspace_size": (sz, [i64, i32, i64, i32]),
         "gsb_codebook_backward": (C.c_int, [i32, i32, i64, i32, i64, i32, p, i64, p, i32, p, f32, p, p, p, p, p, sz,
                                             p]),
-        "gsb_code_log_probs_forward": (C.c_int, [i32, i64, i64, p, i64, p, i32, i32, p, p, p, p, p, p, p]),
+        "gsb_code_log_probs_workspace_size": (sz, [i64, i64, i32]),
+        "gsb_code_log_probs_forward": (C.c_int, [i32, i64, i64, p, i64, p, i32, i32, p, p, p, p, p, p, p, sz, p]),
         "gsb_code_log_probs_backward": (C.c_int, [i32, i64, i64, p, i64, p, i32, i32, p, p, p, p, p, p, p]),
+        "gsb_code_balance_state_floats": (i64, [i64]),
         "gsb_code_balance_workspace_size": (sz, [i64, i64]),
         "gsb_code_balance_forward": (C.c_int, [i32, i64, i64, i32, p, i64, p, i32, p, p, p, p, p, p, sz, p]),
-        "gsb_code_balance_backward": (C.c_int, [i32, i64, i64, p, i64, p, p, p, p, p, p]),
+        "gsb_code_balance_backward": (C.c_int, [i32, i64, i64, p, i64, p, p, p, p, p]),
         "gsb_peer_buffer_alloc": (C.c_int, [sz, C.POINTER(p)]),
         "gsb_peer_buffer_free": (C.c_int, [p]),
         "gsb_peer_handle": (C.c_int, [p, p]),

@@ -90,8 +90,8 @@ class _Balance(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, codes):
-        loss, counts, stats, coef = _ops().code_balance_fwd(logits, codes, True)
-        ctx.save_for_backward(logits, counts, stats, coef)
+        loss, counts, stats, state = _ops().code_balance_fwd(logits, codes, True)
+        ctx.save_for_backward(logits, stats, state)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(counts)
         return loss, counts

@@ -293,11 +293,14 @@ int gsb_codebook_backward(int32_t table_dtype, int32_t out_dtype, int64_t rows, 
  * the top_k (0 .. GSB_CODE_MAX_TOP) largest log probabilities with their codes,
  * ties to the lower code. A logit of -inf has probability 0; a row of nothing
  * else has log probabilities -inf, entropy 0 and gradient 0. stats [rows, 4]
- * (optional) is what the backward reads. */
+ * (optional) is what the backward reads. The workspace may be NULL where its
+ * size is 0. */
+size_t gsb_code_log_probs_workspace_size(int64_t rows, int64_t codebook_rows, int32_t top_k);
 int gsb_code_log_probs_forward(int32_t dtype, int64_t rows, int64_t codebook_rows, const void* logits,
                                int64_t logits_stride, const void* codes, int32_t code_bytes, int32_t top_k,
                                float* log_probs, float* entropy, float* top_log_probs, int32_t* top_codes,
-                               float* stats, uint32_t* status, void* stream);
+                               float* stats, uint32_t* status, void* workspace, size_t workspace_bytes,
+                               void* stream);
 /* Any incoming gradient may be NULL (zeros). g_logits [rows, codebook_rows] of dtype. */
 int gsb_code_log_probs_backward(int32_t dtype, int64_t rows, int64_t codebook_rows, const void* logits,
                                 int64_t logits_stride, const void* codes, int32_t code_bytes, int32_t top_k,
@@ -309,16 +312,18 @@ int gsb_code_log_probs_backward(int32_t dtype, int64_t rows, int64_t codebook_ro
  * and P_c the mean of softmax(logits)_c over the rows that have a code,
  *   loss = codebook_rows * sum_c f_c P_c      (1 for even use; 0 without any code)
  * and counts [codebook_rows] how often each code occurs. The gradient goes to the
- * logits through P; counts are constants. stats [rows, 4] (optional) and coef [1]
- * are what the backward reads. rows * bag < 2^31. */
+ * logits through P; counts are constants. stats [rows, 4] (optional) and state,
+ * gsb_code_balance_state_floats of them on a 16-byte boundary, are what the
+ * backward reads. rows * bag < 2^31. */
+int64_t gsb_code_balance_state_floats(int64_t codebook_rows);
 size_t gsb_code_balance_workspace_size(int64_t rows, int64_t codebook_rows);
 int gsb_code_balance_forward(int32_t dtype, int64_t rows, int64_t codebook_rows, int32_t bag,
                              const void* logits, int64_t logits_stride, const void* codes, int32_t code_bytes,
-                             float* loss, int32_t* counts, float* stats, float* coef, uint32_t* status,
+                             float* loss, int32_t* counts, float* stats, float* state, uint32_t* status,
                              void* workspace, size_t workspace_bytes, void* stream);
 int gsb_code_balance_backward(int32_t dtype, int64_t rows, int64_t codebook_rows, const void* logits,
-                              int64_t logits_stride, const int32_t* counts, const float* stats,
-                              const float* coef, const float* g_loss, void* g_logits, void* stream);
+                              int64_t logits_stride, const float* stats, const float* state,
+                              const float* g_loss, void* g_logits, void* stream);
 
 /* ---- multi-GPU: gradient sum over NVLink peer memory -----------------------
  * No counterpart in the reference, which is single-device. Sums a float buffer

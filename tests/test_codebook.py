@@ -106,7 +106,9 @@ def test_c_entries_refuse_before_any_launch():
     assert bwd() == 3 and bwd(ws=None, n=1 << 20) == 3 and bwd(g=None, n=1 << 20) == 1
     assert bwd(table=None, gw=one, n=1 << 20) == 1
     lp = lambda dt=0, rows=4, c=8, z=one, stride=8, codes=one, cb=4, k=2, lp=one, ent=one, tl=one, tc=one, st=one: \
-        L.gsb_code_log_probs_forward(dt, rows, c, z, stride, codes, cb, k, lp, ent, tl, tc, None, st, None)
+        L.gsb_code_log_probs_forward(dt, rows, c, z, stride, codes, cb, k, lp, ent, tl, tc, None, st, None, 0, None)
+    assert L.gsb_code_log_probs_workspace_size(1000, 512, 4) == 0
+    assert L.gsb_code_log_probs_workspace_size(3, 100000, 4) > 0 and lp(c=100000) == 3
     assert lp(dt=7) == 2 and lp(rows=1 << 31) == 4 and lp(rows=0, z=None) == 0
     for bad in (dict(c=0), dict(cb=1), dict(k=9), dict(k=-1), dict(k=33, c=64), dict(z=None), dict(codes=None),
                 dict(lp=None), dict(ent=None), dict(tl=None), dict(tc=None), dict(st=None), dict(rows=-1)):
@@ -117,15 +119,16 @@ def test_c_entries_refuse_before_any_launch():
         assert lb(**bad) == 1, bad
     n = L.gsb_code_balance_workspace_size(4, 8)
     assert n > 0 and L.gsb_code_balance_workspace_size(-1, 8) == 0
-    bl = lambda rows=4, bag=1, z=one, codes=one, loss=one, cnt=one, coef=one, st=one, ws=one, n=n: \
-        L.gsb_code_balance_forward(0, rows, 8, bag, z, 8, codes, 4, loss, cnt, None, coef, st, ws, n, None)
-    for bad in (dict(bag=0), dict(z=None), dict(codes=None), dict(loss=None), dict(cnt=None), dict(coef=None),
+    assert L.gsb_code_balance_state_floats(8) == 16 and L.gsb_code_balance_state_floats(9) == 24
+    bl = lambda rows=4, bag=1, z=one, codes=one, loss=one, cnt=one, state=one, st=one, ws=one, n=n: \
+        L.gsb_code_balance_forward(0, rows, 8, bag, z, 8, codes, 4, loss, cnt, None, state, st, ws, n, None)
+    for bad in (dict(bag=0), dict(z=None), dict(codes=None), dict(loss=None), dict(cnt=None), dict(state=None),
                 dict(st=None)):
         assert bl(**bad) == 1, bad
     assert bl(ws=None) == 3 and bl(n=n - 1) == 3 and bl(rows=1 << 30, bag=2) == 4
-    bb = lambda z=one, cnt=one, st=one, coef=one, g=one, dz=one: \
-        L.gsb_code_balance_backward(0, 4, 8, z, 8, cnt, st, coef, g, dz, None)
-    for bad in (dict(z=None), dict(cnt=None), dict(st=None), dict(coef=None), dict(g=None), dict(dz=None)):
+    bb = lambda z=one, st=one, state=one, g=one, dz=one: \
+        L.gsb_code_balance_backward(0, 4, 8, z, 8, st, state, g, dz, None)
+    for bad in (dict(z=None), dict(st=None), dict(state=None), dict(g=None), dict(dz=None)):
         assert bb(**bad) == 1, bad
 
 
