@@ -4,7 +4,7 @@
 // sum_c f_c P_c is the mean over the rows of d = sum_c p_c f_c, so no sums over
 // columns are needed: with the counts at hand each row is one weighted softmax sum
 // (code_rows.cuh), read once. The sums of d over rows are 64-bit, in a fixed order.
-#include "code_rows.cuh"
+#include "code_tiles.cuh"
 
 namespace gsb {
 namespace {
@@ -13,10 +13,19 @@ constexpr int kGroupThreads = 256;
 constexpr int kCountBlocks = 2 * 148;
 constexpr int kCountSharedCodes = 8192;  // counts that a block keeps in shared memory
 constexpr int kCountFew = 8192;          // slots that one block counts alone
-constexpr int kBalanceBlocks = 16 * 148;
+constexpr int kBalanceSums = 32 * 148;   // sums over rows, at most
 constexpr int kStateHead = 8;  // floats before the counts in `state`; [0]: C / (rows with a code x codes counted)
 
 __host__ __device__ inline int64_t padded(int64_t codes) { return (codes + 7) / 8 * 8; }
+
+// Where the counts are as floats: `state` behind its head, in the two layouts of Counts.
+__host__ __device__ inline Counts counts_of(const float* state, int64_t codes) {
+  return Counts{state + kStateHead, state + kStateHead + padded(codes), padded(codes) / 8};
+}
+__device__ __forceinline__ void put_count(float* state, int64_t codes, int64_t c, float n) {
+  state[kStateHead + c] = n;
+  state[kStateHead + padded(codes) + (c & 7) * (padded(codes) / 8) + (c >> 3)] = n;
+}
 
 struct CountParts {  // of each block of the counting kernel: codes counted, rows with one
   uint32_t* codes = nullptr;
@@ -42,7 +51,7 @@ __device__ __forceinline__ V block_total(V v, V* s_warp) {
 template <bool kShared, bool kAlone>
 __global__ void __launch_bounds__(512)
     k_code_counts(int64_t rows, int bag, int C, Codes codes, int32_t* __restrict__ counts,
-                  float* __restrict__ counts_f32, CountParts parts, uint32_t* status) {
+                  float* __restrict__ state, CountParts parts, uint32_t* status) {
   pdl_wait();
   pdl_trigger();
   extern __shared__ int s_count[];
@@ -75,20 +84,20 @@ __global__ void __launch_bounds__(512)
   if constexpr (kShared) {
     for (int c = threadIdx.x; c < C; c += blockDim.x) {
       const int v = s_count[c];
-      if constexpr (kAlone) counts[c] = v, counts_f32[c] = (float)v;
+      if constexpr (kAlone) counts[c] = v, put_count(state, C, c, (float)v);
       else if (v) atomicAdd(&counts[c], v);
     }
     if constexpr (kAlone)
-      for (int c = C + threadIdx.x; c < (int)padded(C); c += blockDim.x) counts_f32[c] = 0.0f;
+      for (int c = C + threadIdx.x; c < (int)padded(C); c += blockDim.x) put_count(state, C, c, 0.0f);
   }
 }
 
 __global__ void __launch_bounds__(256)
-    k_counts_f32(int64_t C, const int32_t* __restrict__ counts, float* __restrict__ counts_f32) {
+    k_counts_f32(int64_t C, const int32_t* __restrict__ counts, float* __restrict__ state) {
   pdl_wait();
   pdl_trigger();
   const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c < padded(C)) counts_f32[c] = c < C ? (float)counts[c] : 0.0f;
+  if (c < padded(C)) put_count(state, C, c, c < C ? (float)counts[c] : 0.0f);
 }
 
 // Whether a row has a code; `width` lanes look.
@@ -115,73 +124,55 @@ __device__ __forceinline__ float finish(RowStat r, bool valid, float4* stats) {
   return out ? 0.0f : r.n + dr;
 }
 
-// Rows of up to 512 codes: L lanes each.
-template <typename T, int VEC, int L>
-__global__ void __launch_bounds__(kGroupThreads)
-    k_balance_group(int64_t rows, int C, int bag, const T* __restrict__ logits, int64_t stride, Codes codes,
-                    const float* __restrict__ counts, float4* __restrict__ stats, double* __restrict__ sums) {
+// parts > 1: a part's sums go to `stat` and `stat_a` for k_balance_join.
+template <typename T, int L>
+__global__ void __launch_bounds__(kTileWarps * 32)
+    k_balance(TileRows<T> t, int bag, Codes codes, Counts counts, float4* __restrict__ stats,
+              float4* __restrict__ stat, uint32_t* __restrict__ stat_a, double* __restrict__ sums) {
   pdl_wait();
   pdl_trigger();
-  __shared__ double s_warp[kGroupThreads / 32];
-  constexpr int kRows = kGroupThreads / L;
-  const int lane = threadIdx.x % L;
+  __shared__ uint4 s_buf[kTileWarps][kTileStages * kTilePieces * 32];
+  const int warp = threadIdx.x / 32, lane32 = threadIdx.x % 32, lane = lane32 % L;
+  int64_t next_code = -1, code = -1;  // one of the row's; a lane takes more only where there are more than lanes
+  RowStat row;
   double sum = 0.0;
-  for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < rows; row0 += (int64_t)gridDim.x * kRows) {
-    const int64_t mine = row0 + threadIdx.x / L;
-    const bool on = mine < rows;
-    const int64_t row = on ? mine : rows - 1;  // lanes without a row keep a warp's exchanges whole
-    float z[kRowElems];
-    load_row<VEC>(logits + row * stride, C, L, lane, z);
-    const bool valid = any_code<L>(codes, row, bag, C, lane);
-    const RowStat r = row_stat<VEC, L, true>(z, C, L, lane, counts, [&](int c) { return counts[c]; });
-    if (on && lane == 0) sum += (double)finish(r, valid, stats ? stats + row : nullptr);
-  }
-  sum = block_total(sum, s_warp);
-  if (threadIdx.x == 0) sums[blockIdx.x] = sum;
-}
-
-// One block of W warps per stretch; parts > 1: its sums go to `stat` for k_balance_join.
-template <typename T, int VEC, int W>
-__global__ void __launch_bounds__(W * 32)
-    k_balance_block(int64_t items, int64_t C, int bag, int parts, int part_len, const T* __restrict__ logits,
-                    int64_t stride, Codes codes, const float* __restrict__ counts, float4* __restrict__ stats,
-                    float4* __restrict__ stat, uint32_t* __restrict__ stat_a, double* __restrict__ sums) {
-  pdl_wait();
-  pdl_trigger();
-  __shared__ RowStat s_stat[2][W];
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  double sum = 0.0;
-  int turn = 0;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x, turn ^= 1) {
-    const int64_t row = parts == 1 ? item : item / parts;
-    const int c0 = (int)(item - row * parts) * part_len;
-    const int len = (int)min((int64_t)part_len, C - c0);
-    float z[kRowElems];
-    load_row<VEC>(logits + row * stride + c0, len, W * 32, tid, z);
-    const bool valid = warp == 0 && parts == 1 && any_code<32>(codes, row, bag, C, lane);
-    const float* n = counts + c0;
-    RowStat r = row_stat<VEC, 32, true>(z, len, W * 32, tid, n, [&](int c) { return n[c]; });
-    r.a += (uint32_t)c0;
-    if (W > 1) {
-      // Two buffers: a warp writes the next stretch's while warp 0 may still read this one's.
-      if (lane == 0) s_stat[turn][warp] = r;
-      __syncthreads();
-      if (warp == 0) {
-        r = s_stat[turn][lane % W];
+  walk_tiles<T, L>(
+      t, s_buf[warp], lane32,
+      [&](const TilePlace<T, L>& next) {
+        next_code = lane < bag ? codes.at(next.row * bag + lane) : -1;
+      },
+      [&] { code = next_code; },
+      [&](const TilePlace<T, L>& now, uint4* buf) {
+        RowStat r = lane_sums<true>(buf, now.values(lane32), counts.from(now.c0));
+        if (L == 32) {
+          if (r.a != 0xffffffffu) r.a += (uint32_t)now.c0;
+          row = now.slice == 0 ? r : join<true>(row, r);
+          if (now.slice + 1 < now.slices) return;
+          r = row;
+        }
 #pragma unroll
-        for (int d = W / 2; d > 0; d >>= 1) r = shuffle_join<true>(r, d, W);
-      }
-    }
-    if (tid == 0) {
-      if (parts == 1) {
-        sum += (double)finish(r, valid, stats ? stats + row : nullptr);
-      } else {
-        stat[item] = make_float4(r.m, r.s, r.w, r.n);
-        stat_a[item] = r.a;
-      }
-    }
+        for (int d = L / 2; d > 0; d >>= 1) r = shuffle_join<true>(r, d, L);
+        int valid = code >= 0 && code < t.codes;
+        for (int j = lane + L; j < bag; j += L) {
+          const int64_t c = codes.at(now.row * bag + j);
+          valid |= c >= 0 && c < t.codes;
+        }
+#pragma unroll
+        for (int d = L / 2; d > 0; d >>= 1) valid |= __shfl_xor_sync(kFullMask, valid, d, L);
+        if (lane == 0) {
+          if (L < 32 || t.parts == 1) {
+            if (now.on) sum += (double)finish(r, valid, stats ? stats + now.row : nullptr);
+          } else {
+            stat[now.item] = make_float4(r.m, r.s, r.w, r.n);
+            stat_a[now.item] = r.a;
+          }
+        }
+      });
+  if (t.parts == 1) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFullMask, sum, d);
+    if (lane32 == 0) sums[blockIdx.x * kTileWarps + warp] = sum;
   }
-  if (parts == 1 && tid == 0) sums[blockIdx.x] = sum;
 }
 
 // A warp per row joins its stretches' sums.
@@ -228,40 +219,50 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// dz_c = g coef p_c ((n_c - n_a) - dr)
-template <typename T, int VEC>
-__device__ __forceinline__ void balance_grad(float k, float4 st, int len, int lanes, int lane, bool on,
-                                             const T* __restrict__ p, const float* __restrict__ counts,
-                                             T* __restrict__ dz) {
+// dz_c = g coef p_c ((n_c - n_a) - dr); `at` deals out the result's values (SAME: the
+// logits' lie alike).
+template <bool SAME, typename T, Mode M>
+__device__ __forceinline__ void balance_grad(float k, float4 st, const Deal<T, M>& at, bool on,
+                                             const T* __restrict__ p, const Counts& counts, T* __restrict__ dz) {
   float z[kRowElems];
-  load_row<VEC>(p, len, lanes, lane, z);
-  const float f = k * st.y;
-  constexpr int P = VEC == 1 ? 1 : 4;  // counts that one load brings
+  if constexpr (SAME) load_row(p, at, 0u, z);
+  else load_row_single(p, at, z);
+  const Base base(st.x);
+  if (__any_sync(kFullMask, base.far)) {
+    const float f = k * st.y;
 #pragma unroll
-  for (int k0 = 0; k0 < kRowElems; k0 += P) {
-    float n[P];
-    const int c = row_index<VEC>(lanes, lane, k0);
-    if constexpr (P == 4) {
-      const float4 q = c < len ? *reinterpret_cast<const float4*>(counts + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-      n[0] = q.x, n[1] = q.y, n[2] = q.z, n[3] = q.w;
-    } else {
-      n[0] = c < len ? counts[c] : 0.0f;
+    for (int i = 0; i < kRowElems; i += 4) {
+      float n[4];
+      counts.four(at, i, n);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float e = ex2_approx((z[i + j] - st.x) * kLog2e);
+        // Takes no part where st.y is 0 (m may be -inf).
+        z[i + j] = st.y == 0.0f ? 0.0f : f * e * ((n[j] - st.w) - st.z);
+      }
     }
+  } else {
+    const F2 l2 = f2(kLog2e), neg_M = f2(base.neg_M), neg_n = f2(-st.w), neg_dr = f2(-st.z),
+             f = f2(k * st.y * base.undo);
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const float e = ex2_approx((z[k0 + i] - st.x) * kLog2e);
-      z[k0 + i] = f * e * ((n[i] - st.w) - st.z);
+    for (int i = 0; i < kRowElems; i += 4) {
+      if (!at.any(i)) continue;
+      float n[4];
+      counts.four(at, i, n);
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        float y0, y1;
+        split(fma2(f2(z[i + j], z[i + j + 1]), l2, neg_M), y0, y1);
+        const F2 e = mul2(f2(ex2_approx(y0), ex2_approx(y1)), f);
+        split(mul2(e, add2(add2(f2(n[j], n[j + 1]), neg_n), neg_dr)), z[i + j], z[i + j + 1]);
+      }
     }
   }
-  if (st.y == 0.0f) {  // takes no part (m may be -inf)
-#pragma unroll
-    for (int i = 0; i < kRowElems; ++i) z[i] = 0.0f;
-  }
-  if (on) store_row<VEC>(dz, len, lanes, lane, z);
+  if (on) store_row(dz, at, z);
 }
 
-template <typename T, int VEC, int L>
-__global__ void __launch_bounds__(kGroupThreads)
+template <typename T, Mode M, bool SAME, int L>
+__global__ void __launch_bounds__(kGroupThreads, kRowThreadsSM / kGroupThreads)
     k_balance_bwd_group(int64_t rows, int C, const T* __restrict__ logits, int64_t stride,
                         const float4* __restrict__ stats, const float* __restrict__ state,
                         const float* __restrict__ g_loss, T* __restrict__ g_logits) {
@@ -271,12 +272,13 @@ __global__ void __launch_bounds__(kGroupThreads)
   const int64_t mine = ((int64_t)blockIdx.x * kGroupThreads + threadIdx.x) / L;
   const bool on = mine < rows;
   const int64_t row = on ? mine : rows - 1;
-  balance_grad<T, VEC>(k, stats[row], C, L, threadIdx.x % L, on, logits + row * stride, state + kStateHead,
-                       g_logits + row * C);
+  T* dz = g_logits + row * C;
+  balance_grad<SAME>(k, stats[row], Deal<T, M>(C, L, threadIdx.x % L, dz), on, logits + row * stride,
+                     counts_of(state, C), dz);
 }
 
-template <typename T, int VEC, int W>
-__global__ void __launch_bounds__(W * 32)
+template <typename T, Mode M, bool SAME, int W>
+__global__ void __launch_bounds__(W * 32, kRowThreadsSM / (W * 32))
     k_balance_bwd_block(int64_t items, int64_t C, int parts, int part_len, const T* __restrict__ logits,
                         int64_t stride, const float4* __restrict__ stats, const float* __restrict__ state,
                         const float* __restrict__ g_loss, T* __restrict__ g_logits) {
@@ -287,8 +289,9 @@ __global__ void __launch_bounds__(W * 32)
     const int64_t row = parts == 1 ? item : item / parts;
     const int c0 = (int)(item - row * parts) * part_len;
     const int len = (int)min((int64_t)part_len, C - c0);
-    balance_grad<T, VEC>(k, stats[row], len, W * 32, threadIdx.x, true, logits + row * stride + c0,
-                         state + kStateHead + c0, g_logits + row * C + c0);
+    T* dz = g_logits + row * C + c0;
+    balance_grad<SAME>(k, stats[row], Deal<T, M>(len, W * 32, threadIdx.x, dz), true, logits + row * stride + c0,
+                       counts_of(state, C).from(c0), dz);
   }
 }
 
@@ -298,12 +301,12 @@ struct BalanceScratch {
   float4* stat = nullptr;
   uint32_t* stat_a = nullptr;
 };
-BalanceScratch carve(Carver& ws, int64_t rows, const RowPlan& plan) {
+BalanceScratch carve(Carver& ws, int64_t rows, const TilePlan& plan) {
   BalanceScratch b;
   b.count.codes = ws.take<uint32_t>(kCountBlocks);
   b.count.rows = ws.take<uint32_t>(kCountBlocks);
-  b.sums = ws.take<double>(kBalanceBlocks);
-  if (plan.lanes == 0 && plan.parts > 1) {
+  b.sums = ws.take<double>(kBalanceSums);
+  if (plan.parts > 1) {
     b.stat = ws.take<float4>((size_t)rows * plan.parts);
     b.stat_a = ws.take<uint32_t>((size_t)rows * plan.parts);
   }
@@ -316,14 +319,20 @@ BalanceScratch carve(Carver& ws, int64_t rows, const RowPlan& plan) {
 using namespace gsb;
 
 extern "C" int64_t gsb_code_balance_state_floats(int64_t codebook_rows) {
-  return codebook_rows <= 0 ? 0 : kStateHead + padded(codebook_rows);
+  return codebook_rows <= 0 ? 0 : kStateHead + 2 * padded(codebook_rows);
 }
 
 extern "C" size_t gsb_code_balance_workspace_size(int64_t rows, int64_t codebook_rows) {
   if (check_rows(GSB_DTYPE_F32, rows, codebook_rows, 0, 4) != GSB_OK) return 0;
-  Carver c(nullptr);
-  carve(c, rows, row_plan(std::max<int64_t>(rows, 1), codebook_rows));
-  return c.off;
+  size_t need = 0;
+  for (int size = 2; size <= 4; size += 2) {
+    for (int shifted = 0; shifted < 2; ++shifted) {
+      Carver c(nullptr);
+      carve(c, rows, tile_plan(std::max<int64_t>(rows, 1), codebook_rows, size, shifted));
+      need = std::max(need, c.off);
+    }
+  }
+  return need;
 }
 
 extern "C" int gsb_code_balance_forward(int32_t dtype, int64_t rows, int64_t codebook_rows, int32_t bag,
@@ -338,66 +347,56 @@ extern "C" int gsb_code_balance_forward(int32_t dtype, int64_t rows, int64_t cod
   if (!workspace || workspace_bytes < gsb_code_balance_workspace_size(rows, codebook_rows)) return GSB_ERR_WORKSPACE;
   if (rows == 1) logits_stride = 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const RowPlan plan = row_plan(std::max<int64_t>(rows, 1), codebook_rows);
+  const TilePlan plan = tile_plan(std::max<int64_t>(rows, 1), codebook_rows, dtype_bytes(dtype),
+                                  rows_shifted(dtype_bytes(dtype), logits, logits_stride));
   Carver ws(workspace);
   const BalanceScratch b = carve(ws, rows, plan);
   const Codes cd{codes, code_bytes == 8};
-  float* counts_f32 = state + kStateHead;
+  const Counts counts_f32 = counts_of(state, codebook_rows);
   // The counts.
   const bool shared = codebook_rows <= kCountSharedCodes;
   const int64_t slots = rows * bag;
   unsigned count_blocks = 1;
   if (shared && slots <= kCountFew) {
     launch_pdl(k_code_counts<true, true>, 1, 512, sizeof(int) * (size_t)codebook_rows, s, rows, bag,
-               (int)codebook_rows, cd, counts, counts_f32, b.count, status);
+               (int)codebook_rows, cd, counts, state, b.count, status);
     note_launches(1);
   } else {
     if (cudaMemsetAsync(counts, 0, sizeof(int32_t) * (size_t)codebook_rows, s) != cudaSuccess) return GSB_ERR_CUDA;
     count_blocks = (unsigned)std::min<int64_t>(kCountBlocks, grid1d(rows, 512));
     if (shared)
       launch_pdl(k_code_counts<true, false>, count_blocks, 512, sizeof(int) * (size_t)codebook_rows, s, rows, bag,
-                 (int)codebook_rows, cd, counts, counts_f32, b.count, status);
+                 (int)codebook_rows, cd, counts, state, b.count, status);
     else
       launch_pdl(k_code_counts<false, false>, count_blocks, 512, 0, s, rows, bag, (int)codebook_rows, cd, counts,
-                 counts_f32, b.count, status);
+                 state, b.count, status);
     launch_pdl(k_counts_f32, grid1d(padded(codebook_rows), 256), 256, 0, s, codebook_rows, (const int32_t*)counts,
-               counts_f32);
+               state);
     note_launches(2);
   }
   // The rows.
-  int blocks = 0;
+  int n_sums = 0;
   if (rows > 0) {
-    with_rows(dtype, rows_wide(dtype, logits, logits_stride), [&](auto t, auto vec) {
-      using T = decltype(t);
-      constexpr int VEC = decltype(vec)::value;
-      const T* z = (const T*)logits;
-      if (plan.lanes > 0) {
-        with_lanes(plan.lanes, [&](auto l) {
-          constexpr int L = decltype(l)::value;
-          blocks = std::min(kBalanceBlocks, grid1d(rows * L, kGroupThreads));
-          launch_pdl(k_balance_group<T, VEC, L>, blocks, kGroupThreads, 0, s, rows, (int)codebook_rows, bag, z,
-                     logits_stride, cd, (const float*)counts_f32, (float4*)stats, b.sums);
-        });
-      } else {
-        with_warps(plan.warps, [&](auto w) {
-          constexpr int W = decltype(w)::value;
-          const int64_t items = rows * plan.parts;
-          blocks = (int)std::min<int64_t>(plan.parts == 1 ? kBalanceBlocks : (int64_t(1) << 31) - 1, items);
-          launch_pdl(k_balance_block<T, VEC, W>, blocks, W * 32, 0, s, items, codebook_rows, bag, plan.parts,
-                     plan.part_len, z, logits_stride, cd, (const float*)counts_f32, (float4*)stats, b.stat, b.stat_a,
-                     b.sums);
-        });
-        if (plan.parts > 1) {
-          blocks = std::min(kBalanceBlocks, grid1d(rows, 4));
-          launch_pdl(k_balance_join, blocks, 128, 0, s, rows, codebook_rows, bag, plan.parts, cd,
-                     (const float4*)b.stat, (const uint32_t*)b.stat_a, (float4*)stats, b.sums);
-          note_launches(1);
-        }
-      }
+    with_dtype(dtype, [&](auto tag) {
+      using T = decltype(tag);
+      const int64_t items = plan.items(rows);
+      const TileRows<T> t{(const T*)logits, logits_stride, rows, codebook_rows, plan.part_len, items, plan.parts};
+      const int blocks = tile_blocks(items);
+      n_sums = blocks * kTileWarps;
+      with_tile_lanes(plan.lanes, [&](auto l) {
+        launch_pdl(k_balance<T, decltype(l)::value>, blocks, kTileWarps * 32, 0, s, t, bag, cd, counts_f32,
+                   (float4*)stats, b.stat, b.stat_a, b.sums);
+      });
     });
     note_launches(1);
+    if (plan.parts > 1) {
+      n_sums = std::min(kBalanceSums, grid1d(rows, 4));
+      launch_pdl(k_balance_join, n_sums, 128, 0, s, rows, codebook_rows, bag, plan.parts, cd, (const float4*)b.stat,
+                 (const uint32_t*)b.stat_a, (float4*)stats, b.sums);
+      note_launches(1);
+    }
   }
-  launch_pdl(k_balance_loss, 1, 256, 0, s, blocks, codebook_rows, (const double*)b.sums, (int)count_blocks, b.count,
+  launch_pdl(k_balance_loss, 1, 256, 0, s, n_sums, codebook_rows, (const double*)b.sums, (int)count_blocks, b.count,
              loss, state);
   note_launches(1);
   return cuda_status(cudaGetLastError());
@@ -410,27 +409,26 @@ extern "C" int gsb_code_balance_backward(int32_t dtype, int64_t rows, int64_t co
   if (rc != GSB_OK) return rc;
   if (rows == 0) return GSB_OK;
   if (!logits || !stats || !state || !g_loss || !g_logits) return GSB_ERR_INVALID_ARGUMENT;
-  if (rows == 1) logits_stride = 0;
-  const RowPlan plan = row_plan(rows, codebook_rows);
+  if (rows == 1) logits_stride = codebook_rows;  // as the result's
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // Wide pieces where both the logits' and the gradient's rows are whole ones.
-  const bool wide = rows_wide(dtype, logits, logits_stride) && rows_wide(dtype, g_logits, codebook_rows);
-  with_rows(dtype, wide, [&](auto t, auto vec) {
+  with_row_pairs(dtype, logits, logits_stride, g_logits, codebook_rows, [&](auto t, auto m, auto same) {
     using T = decltype(t);
-    constexpr int VEC = decltype(vec)::value;
+    constexpr Mode M = decltype(m)::value;
+    constexpr bool SAME = decltype(same)::value;
+    const RowPlan plan = row_plan(rows, codebook_rows, M == Mode::kShifted);
     if (plan.lanes > 0) {
       with_lanes(plan.lanes, [&](auto l) {
         constexpr int L = decltype(l)::value;
-        launch_pdl(k_balance_bwd_group<T, VEC, L>, grid1d(rows * L, kGroupThreads), kGroupThreads, 0, s, rows,
+        launch_pdl(k_balance_bwd_group<T, M, SAME, L>, grid1d(rows * L, kGroupThreads), kGroupThreads, 0, s, rows,
                    (int)codebook_rows, (const T*)logits, logits_stride, (const float4*)stats, state, g_loss,
                    (T*)g_logits);
       });
     } else {
       with_warps(plan.warps, [&](auto w) {
         constexpr int W = decltype(w)::value;
-        launch_pdl(k_balance_bwd_block<T, VEC, W>, item_grid(rows * plan.parts), W * 32, 0, s, rows * plan.parts,
-                   codebook_rows, plan.parts, plan.part_len, (const T*)logits, logits_stride, (const float4*)stats,
-                   state, g_loss, (T*)g_logits);
+        launch_pdl(k_balance_bwd_block<T, M, SAME, W>, item_grid(rows * plan.parts), W * 32, 0, s,
+                   rows * plan.parts, codebook_rows, plan.parts, plan.part_len, (const T*)logits, logits_stride,
+                   (const float4*)stats, state, g_loss, (T*)g_logits);
       });
     }
   });

@@ -3,13 +3,12 @@
 //
 // A -inf logit has probability 0. In a row of -inf only log p is -inf, H and the
 // gradient are 0. NaN or +inf make a row's results NaN.
-#include "code_rows.cuh"
+#include "code_tiles.cuh"
 
 namespace gsb {
 namespace {
 
 constexpr int kGroupThreads = 256;
-constexpr int kTopList = 256;  // candidates for the alternatives that a block can rank
 
 struct LogProbsOut {
   float *log_probs, *entropy, *top_log_probs;
@@ -43,210 +42,217 @@ __device__ __forceinline__ int64_t given_code(const LogProbsOut& o, const Codes&
   return c < C ? c : -1;
 }
 
-// Rows of up to 512 codes: L lanes each. The alternatives come one by one: the
-// largest of what is left, taken out of its lane's registers (NaN, which loses
-// against any number).
-template <typename T, int VEC, int L>
-__global__ void __launch_bounds__(kGroupThreads)
-    k_log_probs_group(int64_t rows, int C, const T* __restrict__ logits, int64_t stride, Codes codes, int top_k,
-                      LogProbsOut o, uint32_t* status) {
-  pdl_wait();
-  pdl_trigger();
-  const int lane = threadIdx.x % L;
-  const int64_t mine = ((int64_t)blockIdx.x * kGroupThreads + threadIdx.x) / L;
-  const bool on = mine < rows;
-  const int64_t row = on ? mine : rows - 1;  // lanes without a row keep a warp's exchanges whole
-  const T* p = logits + row * stride;
-  float z[kRowElems];
-  load_row<VEC>(p, C, L, lane, z);
-  const int64_t code = given_code(o, codes, row, C, on && lane == 0, status);
-  const float zc = code >= 0 ? to_f32(p[code]) : 0.0f;
-  RowStat r = row_stat<VEC, L, false>(z, C, L, lane, nullptr, [](int) { return 0.0f; });
-  const RowResult q = finish(r);
-  if (on && lane == 0) write_row(o, row, r, q, code, code >= 0, zc);
-  if (top_k == 0) return;
-  uint32_t a = r.a, taken = 0;  // taken: a bit for each of the lane's values
-  float best = r.m, top = 0.0f;
-  int at = 0;  // the lane's own largest, and where it is
+// Alternatives of a row that L lanes have in `buf` (a slice holds it all), one by
+// one: every lane has its own largest, taken out of the buffer; the row's largest of
+// those is next, and its lane looks for another.
+template <typename T, int L>
+__device__ __forceinline__ void pick_alternatives(uint4* buf, int lane, const TilePlace<T, L>& now,
+                                                  const Slice<T, L>& at, const RowStat& own, const RowResult& q,
+                                                  const LogProbsOut& o, int top_k) {
+  constexpr int VEC = wide_of<T>();
+  uint64_t best = own.a == 0xffffffffu ? 0 : order_key(own.m, own.a);
+  int nan_from = 0;
+  // What is out is NaN from here on.
+  auto take = [&](int c) {
+    const int k = c - at.first;  // pieces lie L VEC apart
+    reinterpret_cast<T*>(buf + k / (L * VEC) * 32)[k % (L * VEC)] = from_f32<T>(quiet_nan());
+  };
+  if (at.ragged()) fill_ragged(buf, at, quiet_nan());
+  if (best != 0) take((int)own.a);
   for (int j = 0;; ++j) {
-    if (on && lane == 0) {
-      o.top_codes[row * top_k + j] = (int32_t)a;
-      o.top_log_probs[row * top_k + j] = q.log_p(best);
+    uint64_t row_best = best;
+#pragma unroll
+    for (int d = L / 2; d > 0; d >>= 1) {
+      const uint64_t u = __shfl_xor_sync(kFullMask, row_best, d, L);
+      row_best = u > row_best ? u : row_best;
+    }
+    if (now.on && lane == 0) {
+      uint32_t c = key_index(row_best);
+      float z = key_value(row_best);
+      if (row_best == 0) {  // NaN alone is left, from the lowest index on
+        while (nan_from < at.len - 1 && to_f32(now.p[nan_from]) == to_f32(now.p[nan_from])) ++nan_from;
+        c = (uint32_t)nan_from++;
+        z = quiet_nan();
+      }
+      o.top_codes[now.row * top_k + j] = (int32_t)c;
+      o.top_log_probs[now.row * top_k + j] = q.log_p(z);
     }
     if (j + 1 == top_k) break;
-    if (j == 0) {  // places behind the row's end are never taken
+    if (best == row_best && best != 0) {
+      float top = quiet_nan();
+      int top_v = 0;
 #pragma unroll
-      for (int k = 0; k < kRowElems; ++k)
-        if (row_index<VEC>(L, lane, k) >= C) z[k] = quiet_nan(), taken |= 1u << k;
+      for (int v = 0; v < kTilePieces; ++v) {
+        if (v < at.n) {
+          float hi, lo;
+          piece_range(buf[v * 32], T{}, hi, lo);
+          if (hi == hi && !(hi <= top)) top = hi, top_v = v;  // the first of equal ones
+        }
+      }
+      best = 0;
+      if (top == top) {
+        float f[VEC];
+        unpack<T>(buf[top_v * 32], f);
+        int c = 0;
+#pragma unroll
+        for (int i = VEC - 1; i >= 0; --i)
+          if (f[i] == top) c = at.at(top_v) + i;
+        best = order_key(top, (uint32_t)c);
+        take(c);
+      }
     }
-    const bool owner = (int)(a / VEC) % L == lane;
-    if (owner || j == 0) {
-      const int out = owner ? (int)(a / (VEC * L)) * VEC + (int)a % VEC : kRowElems;
-      if (owner) taken |= 1u << out;
-#pragma unroll
-      for (int k = 0; k < kRowElems; ++k)
-        if (k == out) z[k] = quiet_nan();
-      top = lane_max(z);
-      at = kRowElems;
-#pragma unroll
-      for (int k = kRowElems - 1; k >= 0; --k)
-        if (z[k] == top) at = k;
-    }
-    best = top;
-#pragma unroll
-    for (int d = L / 2; d > 0; d >>= 1) best = fmaxf(best, __shfl_xor_sync(kFullMask, best, d, L));
-    // NaN: nothing but NaN is left, taken from the lowest index on.
-    const int pick = best != best ? __ffs(~taken) - 1 : (top == best ? at : -1);
-    a = pick >= 0 && pick < kRowElems ? (uint32_t)row_index<VEC>(L, lane, pick) : 0x7fffffffu;
-#pragma unroll
-    for (int d = L / 2; d > 0; d >>= 1) a = min(a, __shfl_xor_sync(kFullMask, a, d, L));
   }
 }
 
-// Block-wide largest key below `limit` among the registers' values.
-template <int VEC, int W>
-__device__ __forceinline__ uint64_t block_best(const float (&z)[kRowElems], int len, int c0, uint64_t limit,
-                                               uint64_t* s_key) {
-  uint64_t best = 0;
-#pragma unroll
-  for (int k = 0; k < kRowElems; ++k) {
-    const int c = row_index<VEC>(W * 32, threadIdx.x, k);
-    const uint64_t key = order_key(z[k], (uint32_t)(c0 + c));
-    if (c < len && key < limit && key > best) best = key;
+// The k largest keys of a part of a row, to put(rank, key). k lanes hold a value of
+// at least the k-th largest of the lanes' maxima, so none of the k largest is below
+// that; the slices of lanes that reach it are read again (they come from L2) and the
+// few values that do are listed and ranked against one another. Many equal values can
+// overrun the list: then the part is searched once for each key.
+constexpr int kTopList = 128;
+template <typename T, typename Put>
+__device__ __forceinline__ void list_alternatives(const TilePlace<T, 32>& now, int lane, float lane_best, int k,
+                                                  const float (*top)[32], uint64_t* list, int* count, Put&& put) {
+  constexpr int VEC = wide_of<T>();
+  uint32_t left = order_bits(lane_best), bound = 0;
+  for (int j = 0; j < k; ++j) {
+    bound = __reduce_max_sync(kFullMask, left);
+    const uint32_t who = __ballot_sync(kFullMask, left == bound);
+    if (lane == __ffs(who) - 1) left = 0;
   }
+  const float least = key_value((uint64_t)bound << 32);
+  if (lane == 0) *count = 0;
+  __syncwarp();
+  for (int j = 0; j < now.slices; ++j) {
+    if (!(top[j][lane] >= least)) continue;
+    const Slice<T, 32> at(now.len, now.shift, j, lane);
+    for (int v = 0; v < kTilePieces; ++v) {
+      const int c = at.at(v);
+      if (c >= at.len) break;
+      float f[VEC];
+      if (c >= 0 && c + VEC <= at.len) {
+        unpack<T>(*reinterpret_cast<const uint4*>(now.p + c), f);
+      } else {
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    const uint64_t u = __shfl_xor_sync(kFullMask, best, d);
-    best = u > best ? u : best;
-  }
-  if (W > 1) {
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) s_key[threadIdx.x / 32] = best;
-    __syncthreads();
+        for (int i = 0; i < VEC; ++i) f[i] = at.has(c + i) ? to_f32(now.p[c + i]) : quiet_nan();
+      }
+      float hi = f[0];
 #pragma unroll
-    for (int w = 0; w < W; ++w) best = s_key[w] > best ? s_key[w] : best;
+      for (int i = 1; i < VEC; ++i) hi = fmaxf(hi, f[i]);
+      if (hi >= least) {
+        for (int i = 0; i < VEC; ++i) {
+          const float z = at.has(c + i) ? to_f32(now.p[c + i]) : quiet_nan();
+          if (z >= least) {
+            const int to = atomicAdd(count, 1);
+            if (to < kTopList) list[to] = order_key(z, (uint32_t)(now.c0 + c + i));
+          }
+        }
+      }
+    }
   }
-  return best;
+  __syncwarp();
+  const int n = *count;
+  if (n >= k && n <= kTopList) {
+    for (int i = lane; i < n; i += 32) {
+      const uint64_t key = list[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += list[j] > key;
+      if (rank < k) put(rank, key);
+    }
+  } else {
+    uint64_t limit = ~uint64_t(0);
+    for (int j = 0; j < k; ++j) {
+      uint64_t best = 0;
+      for (int c = lane; c < now.len; c += 32) {
+        const uint64_t key = order_key(to_f32(now.p[c]), (uint32_t)(now.c0 + c));
+        if (key < limit && key > best) best = key;
+      }
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) {
+        const uint64_t u = __shfl_xor_sync(kFullMask, best, d);
+        best = u > best ? u : best;
+      }
+      limit = best;
+      if (lane == 0) put(j, best);
+    }
+  }
+  __syncwarp();
 }
 
-// One block of W warps per stretch. The alternatives: k lanes hold a value of at
-// least the k-th largest of a warp's lane maxima, so none of the k largest is below
-// the largest of those bounds over the warps; the few values that are not (k and a
-// handful) are listed and ranked against one another. Many equal values can overrun
-// the list: then the alternatives are found one by one. parts > 1: the stretch's
-// sums and keys go to `stat` and `keys` for k_log_probs_join.
-template <typename T, int VEC, int W>
-__global__ void __launch_bounds__(W * 32)
-    k_log_probs_block(int64_t items, int64_t C, int parts, int part_len, const T* __restrict__ logits, int64_t stride,
-                      Codes codes, int top_k, LogProbsOut o, float4* __restrict__ stat, uint64_t* __restrict__ keys,
-                      uint32_t* status) {
+// parts > 1: a part's sums and keys go to `stat` and `keys` for k_log_probs_join.
+template <typename T, int L>
+__global__ void __launch_bounds__(kTileWarps * 32)
+    k_log_probs(TileRows<T> t, Codes codes, int top_k, LogProbsOut o, float4* __restrict__ stat,
+                uint64_t* __restrict__ keys, uint32_t* status) {
   pdl_wait();
   pdl_trigger();
-  __shared__ RowStat s_stat[W];
-  __shared__ uint32_t s_bound[W];
-  __shared__ uint64_t s_list[kTopList];
-  __shared__ uint64_t s_key[W];
-  __shared__ RowResult s_result;
-  __shared__ int s_count;
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int64_t row = parts == 1 ? item : item / parts;
-    const int part = (int)(item - row * parts);
-    const int c0 = part * part_len;
-    const int len = (int)min((int64_t)part_len, C - c0);
-    const T* p = logits + row * stride;
-    float z[kRowElems];
-    load_row<VEC>(p + c0, len, W * 32, tid, z);
-    int64_t code = -1;
-    float zc = 0.0f;
-    if (parts == 1 && warp == 0) {
-      code = given_code(o, codes, row, C, lane == 0, status);
-      zc = code >= 0 ? to_f32(p[code]) : 0.0f;
-    }
-    RowStat r = row_stat<VEC, 32, false>(z, len, W * 32, tid, nullptr, [](int) { return 0.0f; });
-    r.a += (uint32_t)c0;
-    const int k = min(top_k, len);
-    if (k > 1) {
-      uint32_t left = order_bits(lane_max(z)), bound = 0;
-      for (int j = 0; j < k; ++j) {
-        bound = __reduce_max_sync(kFullMask, left);
-        const uint32_t who = __ballot_sync(kFullMask, left == bound);
-        if (lane == __ffs(who) - 1) left = 0;
-      }
-      if (lane == 0) s_bound[warp] = bound;
-    }
-    if (tid == 0) s_count = 0;
-    if (lane == 0) s_stat[warp] = r;
-    __syncthreads();
-    RowResult q;
-    if (warp == 0) {
-      if (W > 1) {
-        r = s_stat[lane % W];
+  __shared__ uint4 s_buf[kTileWarps][kTileStages * kTilePieces * 32];
+  __shared__ float s_top[L == 32 ? kTileWarps : 1][kTileSlices][32];
+  __shared__ uint64_t s_list[L == 32 ? kTileWarps : 1][kTopList];
+  __shared__ int s_count[kTileWarps];
+  const int warp = threadIdx.x / 32, lane32 = threadIdx.x % 32, lane = lane32 % L;
+  int64_t next_code = -1, code = -1;
+  float zc = 0.0f;
+  const bool given = o.log_probs != nullptr && (L < 32 || t.parts == 1);
+  RowStat sums;
+  walk_tiles<T, L>(
+      t, s_buf[warp], lane32,
+      [&](const TilePlace<T, L>& next) {
+        if (given) next_code = codes.at(next.row);
+      },
+      [&] { code = next_code; },
+      [&](const TilePlace<T, L>& now, uint4* buf) {
+        if (now.slice == 0) {
+          if (code >= t.codes) {
+            if (now.on && lane == 0) bad_code(status, kSiteCode);
+            code = -1;
+          }
+          zc = code >= 0 ? to_f32(now.p[code]) : 0.0f;
+        }
+        const Slice<T, L> at = now.values(lane32);
+        RowStat r = lane_sums<false>(buf, at, Counts{});
+        const RowStat own = r;
+        if (L == 32) {
+          if (top_k > 1) s_top[L == 32 ? warp : 0][now.slice][lane32] = r.m;
+          if (r.a != 0xffffffffu) r.a += (uint32_t)now.c0;
+          sums = now.slice == 0 ? r : join<false>(sums, r);
+          if (now.slice + 1 < now.slices) return;
+          r = sums;
+        }
 #pragma unroll
-        for (int d = W / 2; d > 0; d >>= 1) r = shuffle_join<false>(r, d, W);
-      }
-      if (parts == 1) {
-        q = finish(r);
-        if (lane == 0) {
-          write_row(o, row, r, q, code, code >= 0, zc);
-          s_result = q;
-          if (k == 1) {
-            o.top_codes[row] = (int32_t)r.a;
-            o.top_log_probs[row] = q.log_p(r.m);
+        for (int d = L / 2; d > 0; d >>= 1) r = shuffle_join<false>(r, d, L);
+        if (r.a == 0xffffffffu) r.a = (uint32_t)now.c0;  // NaN alone
+        if (L < 32 || t.parts == 1) {
+          const RowResult q = finish(r);
+          if (now.on && lane == 0) {
+            write_row(o, now.row, r, q, code, code >= 0, zc);
+            if (top_k == 1) {
+              o.top_codes[now.row] = (int32_t)r.a;
+              o.top_log_probs[now.row] = q.log_p(r.m);
+            }
+          }
+          if (top_k > 1) {
+            if constexpr (L < 32)
+              pick_alternatives<T, L>(buf, lane, now, at, own, q, o, top_k);
+            else
+              list_alternatives(now, lane32, sums.m, top_k, s_top[warp], s_list[warp], &s_count[warp],
+                                [&](int j, uint64_t key) {
+                                  o.top_codes[now.row * top_k + j] = (int32_t)key_index(key);
+                                  o.top_log_probs[now.row * top_k + j] = q.log_p(key_value(key));
+                                });
+          }
+        } else if constexpr (L == 32) {
+          if (lane32 == 0) stat[now.item] = make_float4(r.m, r.s, r.w, __uint_as_float(r.a));
+          uint64_t* to = keys + now.item * top_k;
+          if (top_k == 1 && lane32 == 0) to[0] = order_key(r.m, r.a);
+          if (top_k > 1) {
+            const int k = min(top_k, now.len);
+            list_alternatives(now, lane32, sums.m, k, s_top[warp], s_list[warp], &s_count[warp],
+                              [&](int j, uint64_t key) { to[j] = key; });
+            for (int j = k + lane32; j < top_k; j += 32) to[j] = 0;  // a short last part
           }
         }
-      } else if (lane == 0) {
-        stat[item] = make_float4(r.m, r.s, r.w, __uint_as_float(r.a));
-        if (k == 1 && top_k == 1) keys[item] = order_key(r.m, r.a);
-      }
-    }
-    if (top_k > 1) {
-      uint32_t bound = 0;
-      if (k > 1) {
-#pragma unroll
-        for (int w = 0; w < W; ++w) bound = max(bound, s_bound[w]);
-      }
-      const float least = key_value((uint64_t)bound << 32);
-#pragma unroll
-      for (int i = 0; i < kRowElems; ++i) {
-        if (z[i] >= least) {
-          const int c = row_index<VEC>(W * 32, tid, i);
-          if (c < len) {
-            const int at = atomicAdd(&s_count, 1);
-            if (at < kTopList) s_list[at] = order_key(z[i], (uint32_t)(c0 + c));
-          }
-        }
-      }
-      __syncthreads();
-      const int count = s_count;
-      auto put = [&](int j, uint64_t key) {
-        if (parts == 1) {
-          const RowResult f = s_result;
-          o.top_codes[row * top_k + j] = (int32_t)key_index(key);
-          o.top_log_probs[row * top_k + j] = f.log_p(key_value(key));
-        } else {
-          keys[item * top_k + j] = key;
-        }
-      };
-      if (count >= k && count <= kTopList) {
-        for (int i = tid; i < count; i += W * 32) {
-          const uint64_t key = s_list[i];
-          int rank = 0;
-          for (int j = 0; j < count; ++j) rank += s_list[j] > key;
-          if (rank < k) put(rank, key);
-        }
-      } else {
-        uint64_t limit = ~uint64_t(0);
-        for (int j = 0; j < k; ++j) {
-          limit = block_best<VEC, W>(z, len, c0, limit, s_key);
-          if (tid == 0) put(j, limit);
-        }
-      }
-      if (parts > 1)
-        for (int j = k + tid; j < top_k; j += W * 32) keys[item * top_k + j] = 0;  // a short last stretch
-    }
-    __syncthreads();
-  }
+      });
 }
 
 // One warp per row joins its stretches' sums and picks the largest keys.
@@ -307,13 +313,16 @@ struct LogProbsIn {
 // dz_c = p_c (-lead - gH (z_c - m - mu)) + sum_i g_i [c = c_i], lead = sum_i g_i over the
 // given code and the alternatives. At the c_i, which are written a second time, the sum
 // is (sum of their g_i) (1 - p_c) - (sum of the other g_i) p_c.
-// `lane` of `lanes` takes its values of a stretch at c0; sync() orders the two writes.
-template <typename T, int VEC, typename Sync>
-__device__ __forceinline__ void log_probs_grad(int64_t row, int64_t C, int c0, int len, int lanes, int lane, bool on,
+// `at` deals out the result's values of a stretch at c0 (SAME: the logits' lie alike);
+// sync() orders the two writes.
+template <bool SAME, typename T, Mode M, typename Sync>
+__device__ __forceinline__ void log_probs_grad(int64_t row, int64_t C, int c0, const Deal<T, M>& at, bool on,
                                                const T* __restrict__ p, T* __restrict__ dz, const LogProbsIn& in,
                                                Sync&& sync) {
+  const int len = at.len, lanes = at.lanes, lane = at.lane;
   float z[kRowElems];
-  load_row<VEC>(p + c0, len, lanes, lane, z);
+  if constexpr (SAME) load_row(p + c0, at, 0u, z);
+  else load_row_single(p + c0, at, z);
   const float4 st = in.stats[row];
   const bool empty = st.x == neg_inf() && st.y == st.y;
   const float inv = 1.0f / (1.0f + st.y);
@@ -328,16 +337,30 @@ __device__ __forceinline__ void log_probs_grad(int64_t row, int64_t C, int c0, i
   for (int j = 0; j < k; ++j) lead += gt[j];
   // p (-lead - gH (x - mu)) = e (alpha + beta x)
   const float beta = -gh * inv, alpha = (gh * st.z - lead) * inv;
+  const Base base(st.x);
+  if (__any_sync(kFullMask, base.far || lane_min(z) < kLowest)) {
 #pragma unroll
-  for (int i = 0; i < kRowElems; ++i) {
-    const float x = max_nan(z[i] - st.x, -200.0f);  // -inf: e is 0, and beta x finite
-    z[i] = ex2_approx(x * kLog2e) * fmaf(beta, x, alpha);
+    for (int i = 0; i < kRowElems; ++i) {
+      const float x = max_nan(z[i] - st.x, -200.0f);  // -inf: e is 0, and beta x finite
+      z[i] = ex2_approx(x * kLog2e) * fmaf(beta, x, alpha);
+    }
+  } else {
+    const float beta2 = beta * kLn2;
+    const F2 l2 = f2(kLog2e), neg_M = f2(base.neg_M), b2 = f2(beta2 * base.undo),
+             a2 = f2((alpha - beta2 * base.d) * base.undo);
+#pragma unroll
+    for (int i = 0; i < kRowElems; i += 2) {
+      const F2 y = fma2(f2(z[i], z[i + 1]), l2, neg_M);
+      float y0, y1;
+      split(y, y0, y1);
+      split(mul2(f2(ex2_approx(y0), ex2_approx(y1)), fma2(b2, y, a2)), z[i], z[i + 1]);
+    }
   }
   if (empty) {
 #pragma unroll
     for (int i = 0; i < kRowElems; ++i) z[i] = 0.0f;
   }
-  if (on) store_row<VEC>(dz + c0, len, lanes, lane, z);
+  if (on) store_row(dz + c0, at, z);
   sync();
   if (!on || empty) return;
   for (int j = lane; j <= k; j += lanes) {
@@ -359,8 +382,8 @@ __device__ __forceinline__ void log_probs_grad(int64_t row, int64_t C, int c0, i
   }
 }
 
-template <typename T, int VEC, int L>
-__global__ void __launch_bounds__(kGroupThreads)
+template <typename T, Mode M, bool SAME, int L>
+__global__ void __launch_bounds__(kGroupThreads, kRowThreadsSM / kGroupThreads)
     k_log_probs_bwd_group(int64_t rows, int C, const T* __restrict__ logits, int64_t stride, LogProbsIn in,
                           T* __restrict__ g_logits) {
   pdl_wait();
@@ -368,12 +391,13 @@ __global__ void __launch_bounds__(kGroupThreads)
   const int64_t mine = ((int64_t)blockIdx.x * kGroupThreads + threadIdx.x) / L;
   const bool on = mine < rows;
   const int64_t row = on ? mine : rows - 1;
-  log_probs_grad<T, VEC>(row, C, 0, C, L, threadIdx.x % L, on, logits + row * stride, g_logits + row * C, in,
-                         [] { __syncwarp(); });
+  T* dz = g_logits + row * C;
+  log_probs_grad<SAME>(row, C, 0, Deal<T, M>(C, L, threadIdx.x % L, dz), on, logits + row * stride, dz, in,
+                       [] { __syncwarp(); });
 }
 
-template <typename T, int VEC, int W>
-__global__ void __launch_bounds__(W * 32)
+template <typename T, Mode M, bool SAME, int W>
+__global__ void __launch_bounds__(W * 32, kRowThreadsSM / (W * 32))
     k_log_probs_bwd_block(int64_t items, int64_t C, int parts, int part_len, const T* __restrict__ logits,
                           int64_t stride, LogProbsIn in, T* __restrict__ g_logits) {
   pdl_wait();
@@ -382,8 +406,9 @@ __global__ void __launch_bounds__(W * 32)
     const int64_t row = parts == 1 ? item : item / parts;
     const int c0 = (int)(item - row * parts) * part_len;
     const int len = (int)min((int64_t)part_len, C - c0);
-    log_probs_grad<T, VEC>(row, C, c0, len, W * 32, threadIdx.x, true, logits + row * stride, g_logits + row * C, in,
-                           [] { __syncthreads(); });
+    T* dz = g_logits + row * C;
+    log_probs_grad<SAME>(row, C, c0, Deal<T, M>(len, W * 32, threadIdx.x, dz + c0), true, logits + row * stride, dz,
+                         in, [] { __syncthreads(); });
   }
 }
 
@@ -391,9 +416,9 @@ struct LogProbsScratch {
   float4* stat = nullptr;
   uint64_t* keys = nullptr;
 };
-LogProbsScratch carve(Carver& ws, int64_t rows, const RowPlan& plan, int top_k) {
+LogProbsScratch carve(Carver& ws, int64_t rows, const TilePlan& plan, int top_k) {
   LogProbsScratch b;
-  if (plan.lanes == 0 && plan.parts > 1) {
+  if (plan.parts > 1) {
     b.stat = ws.take<float4>((size_t)rows * plan.parts);
     b.keys = ws.take<uint64_t>((size_t)rows * plan.parts * top_k);
   }
@@ -413,9 +438,15 @@ using namespace gsb;
 
 extern "C" size_t gsb_code_log_probs_workspace_size(int64_t rows, int64_t codebook_rows, int32_t top_k) {
   if (check_log_probs(GSB_DTYPE_F32, rows, codebook_rows, 0, 4, top_k) != GSB_OK || rows == 0) return 0;
-  Carver c(nullptr);
-  carve(c, rows, row_plan(rows, codebook_rows), top_k);
-  return c.off;
+  size_t need = 0;
+  for (int size = 2; size <= 4; size += 2) {
+    for (int shifted = 0; shifted < 2; ++shifted) {
+      Carver c(nullptr);
+      carve(c, rows, tile_plan(rows, codebook_rows, size, shifted), top_k);
+      need = std::max(need, c.off);
+    }
+  }
+  return need;
 }
 
 extern "C" int gsb_code_log_probs_forward(int32_t dtype, int64_t rows, int64_t codebook_rows, const void* logits,
@@ -432,33 +463,26 @@ extern "C" int gsb_code_log_probs_forward(int32_t dtype, int64_t rows, int64_t c
   const size_t need = gsb_code_log_probs_workspace_size(rows, codebook_rows, top_k);
   if (need > 0 && (!workspace || workspace_bytes < need)) return GSB_ERR_WORKSPACE;
   if (rows == 1) logits_stride = 0;
-  const RowPlan plan = row_plan(rows, codebook_rows);
+  const TilePlan plan = tile_plan(rows, codebook_rows, dtype_bytes(dtype),
+                                  rows_shifted(dtype_bytes(dtype), logits, logits_stride));
   Carver ws(workspace);
   const LogProbsScratch b = carve(ws, rows, plan, top_k);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const Codes cd{codes, code_bytes == 8};
   const LogProbsOut o{log_probs, entropy, top_log_probs, top_codes, (float4*)stats};
-  with_rows(dtype, rows_wide(dtype, logits, logits_stride), [&](auto t, auto vec) {
-    using T = decltype(t);
-    constexpr int VEC = decltype(vec)::value;
-    const T* z = (const T*)logits;
-    if (plan.lanes > 0) {
-      with_lanes(plan.lanes, [&](auto l) {
-        constexpr int L = decltype(l)::value;
-        launch_pdl(k_log_probs_group<T, VEC, L>, grid1d(rows * L, kGroupThreads), kGroupThreads, 0, s, rows,
-                   (int)codebook_rows, z, logits_stride, cd, top_k, o, status);
-      });
-    } else {
-      with_warps(plan.warps, [&](auto w) {
-        constexpr int W = decltype(w)::value;
-        launch_pdl(k_log_probs_block<T, VEC, W>, item_grid(rows * plan.parts), W * 32, 0, s, rows * plan.parts,
-                   codebook_rows, plan.parts, plan.part_len, z, logits_stride, cd, top_k, o, b.stat, b.keys, status);
-      });
-      if (plan.parts > 1) {
-        launch_pdl(k_log_probs_join<T>, grid1d(rows * 32, 128), 128, 0, s, rows, codebook_rows, plan.parts, z,
-                   logits_stride, cd, top_k, (const float4*)b.stat, (const uint64_t*)b.keys, o, status);
-        note_launches(1);
-      }
+  with_dtype(dtype, [&](auto tag) {
+    using T = decltype(tag);
+    const int64_t items = plan.items(rows);
+    const TileRows<T> t{(const T*)logits, logits_stride, rows, codebook_rows, plan.part_len, items, plan.parts};
+    with_tile_lanes(plan.lanes, [&](auto l) {
+      launch_pdl(k_log_probs<T, decltype(l)::value>, tile_blocks(items), kTileWarps * 32, 0, s, t, cd, top_k, o,
+                 b.stat, b.keys, status);
+    });
+    if (plan.parts > 1) {
+      launch_pdl(k_log_probs_join<T>, grid1d(rows * 32, 128), 128, 0, s, rows, codebook_rows, plan.parts,
+                 (const T*)logits, logits_stride, cd, top_k, (const float4*)b.stat, (const uint64_t*)b.keys, o,
+                 status);
+      note_launches(1);
     }
   });
   note_launches(1);
@@ -475,27 +499,27 @@ extern "C" int gsb_code_log_probs_backward(int32_t dtype, int64_t rows, int64_t 
   if (rows == 0) return GSB_OK;
   if (!logits || !stats || !g_logits || (g_log_probs && !codes) || (g_top_log_probs && top_k > 0 && !top_codes))
     return GSB_ERR_INVALID_ARGUMENT;
-  if (rows == 1) logits_stride = 0;
-  const RowPlan plan = row_plan(rows, codebook_rows);
+  if (rows == 1) logits_stride = codebook_rows;  // as the result's
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const LogProbsIn in{Codes{codes, code_bytes == 8}, g_top_log_probs ? top_k : 0, top_codes, (const float4*)stats,
                       g_log_probs, g_entropy, g_top_log_probs};
-  // Wide pieces where both the logits' and the gradient's rows are whole ones.
-  const bool wide = rows_wide(dtype, logits, logits_stride) && rows_wide(dtype, g_logits, codebook_rows);
-  with_rows(dtype, wide, [&](auto t, auto vec) {
+  with_row_pairs(dtype, logits, logits_stride, g_logits, codebook_rows, [&](auto t, auto m, auto same) {
     using T = decltype(t);
-    constexpr int VEC = decltype(vec)::value;
+    constexpr Mode M = decltype(m)::value;
+    constexpr bool SAME = decltype(same)::value;
+    const RowPlan plan = row_plan(rows, codebook_rows, M == Mode::kShifted);
     if (plan.lanes > 0) {
       with_lanes(plan.lanes, [&](auto l) {
         constexpr int L = decltype(l)::value;
-        launch_pdl(k_log_probs_bwd_group<T, VEC, L>, grid1d(rows * L, kGroupThreads), kGroupThreads, 0, s, rows,
+        launch_pdl(k_log_probs_bwd_group<T, M, SAME, L>, grid1d(rows * L, kGroupThreads), kGroupThreads, 0, s, rows,
                    (int)codebook_rows, (const T*)logits, logits_stride, in, (T*)g_logits);
       });
     } else {
       with_warps(plan.warps, [&](auto w) {
         constexpr int W = decltype(w)::value;
-        launch_pdl(k_log_probs_bwd_block<T, VEC, W>, item_grid(rows * plan.parts), W * 32, 0, s, rows * plan.parts,
-                   codebook_rows, plan.parts, plan.part_len, (const T*)logits, logits_stride, in, (T*)g_logits);
+        launch_pdl(k_log_probs_bwd_block<T, M, SAME, W>, item_grid(rows * plan.parts), W * 32, 0, s,
+                   rows * plan.parts, codebook_rows, plan.parts, plan.part_len, (const T*)logits, logits_stride, in,
+                   (T*)g_logits);
       });
     }
   });

@@ -32,6 +32,7 @@ constexpr int kRowElems = 32;          // values a lane
 constexpr int kGroupMaxLanes = 16;     // lanes a row, several rows a warp
 constexpr int kGroupMaxCodes = kGroupMaxLanes * kRowElems;
 constexpr int kBlockMaxWarps = 8;
+constexpr int kRowThreadsSM = 1024;     // threads an SM that registers are kept for (64 each)
 constexpr int kBlockMaxCodes = kBlockMaxWarps * 32 * kRowElems;
 
 __device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
@@ -63,56 +64,79 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 template <typename T>
 constexpr int wide_of() { return 16 / (int)sizeof(T); }
 
+// NaN in every element of a word: a place without a value, which loses against any.
 template <typename T>
-__device__ __forceinline__ uint32_t neg_inf_bits();  // -inf in every element of a word
+__device__ __forceinline__ uint32_t nan_bits();
 template <>
-__device__ __forceinline__ uint32_t neg_inf_bits<float>() { return 0xff800000u; }
+__device__ __forceinline__ uint32_t nan_bits<float>() { return 0x7fc00000u; }
 template <>
-__device__ __forceinline__ uint32_t neg_inf_bits<__nv_bfloat16>() { return 0xff80ff80u; }
+__device__ __forceinline__ uint32_t nan_bits<__nv_bfloat16>() { return 0x7fc07fc0u; }
 template <>
-__device__ __forceinline__ uint32_t neg_inf_bits<__half>() { return 0xfc00fc00u; }
+__device__ __forceinline__ uint32_t nan_bits<__half>() { return 0x7e007e00u; }
 
-// Reads values (v lanes + lane) VEC + i of a stretch of len values, v < kRowElems
-// / VEC, i < VEC, into z[v VEC + i]; -inf behind its end. VEC is 1, or a 16-byte
-// load's worth where the stretch begins on a 16-byte boundary.
-template <int VEC>
-__device__ __forceinline__ int row_index(int lanes, int lane, int k) {
-  return ((k / VEC) * lanes + lane) * VEC + k % VEC;
-}
-template <int VEC, typename T>
-__device__ __forceinline__ void load_row(const T* __restrict__ p, int len, int lanes, int lane,
+// How a stretch of len values of a row is dealt out to `lanes` lanes: lane l's value
+// k has the index (k / VEC lanes + l) VEC + k % VEC - shift. VEC is 1, or the values
+// of a 16-byte piece. shift: values between the 16-byte boundary before the stretch
+// and its start (Mode::kShifted alone), so that pieces lie on boundaries whatever
+// the row's length; the pieces at its ends are read and written by the value.
+enum class Mode { kSingle, kWide, kShifted };
+template <typename T, Mode M>
+struct Deal {
+  static constexpr int VEC = M == Mode::kSingle ? 1 : wide_of<T>();
+  static constexpr bool kShift = M == Mode::kShifted;
+  int len, lanes, lane, shift;
+  __device__ __forceinline__ Deal(int len, int lanes, int lane, const T* p)
+      : len(len), lanes(lanes), lane(lane),
+        shift(kShift ? (int)(reinterpret_cast<uintptr_t>(p) % 16 / sizeof(T)) : 0) {}
+  __device__ __forceinline__ int index(int k) const { return ((k / VEC) * lanes + lane) * VEC + k % VEC - shift; }
+  __device__ __forceinline__ bool has(int c) const { return (!kShift || c >= 0) && c < len; }
+  __device__ __forceinline__ bool whole(int c) const { return (!kShift || c >= 0) && c + VEC <= len; }
+  // False if no lane has anything of its values k, ... of a piece (the same for all lanes).
+  __device__ __forceinline__ bool any(int k) const { return (k / VEC) * lanes * VEC - shift < len; }
+  // Whether all lanes have all of the values k .. k + 3.
+  __device__ __forceinline__ bool all(int k) const {
+    const int last = VEC == 1 ? k + 3 : k / VEC;  // of four values k, ...
+    return (last + 1) * lanes * VEC - shift <= len && (!kShift || k >= VEC || shift == 0);
+  }
+  // The lane and place of index c.
+  __device__ __forceinline__ int lane_of(int c) const { return (c + shift) / VEC % lanes; }
+  __device__ __forceinline__ int place_of(int c) const {
+    return (c + shift) / VEC / lanes * VEC + (c + shift) % VEC;
+  }
+};
+
+// Reads a lane's values; `fill` (the bits of a word of them) where there is none.
+template <typename T, Mode M>
+__device__ __forceinline__ void load_row(const T* __restrict__ p, const Deal<T, M>& at, uint32_t fill,
                                          float (&z)[kRowElems]) {
+  constexpr int VEC = Deal<T, M>::VEC;
   if constexpr (VEC == 1) {
-    T q[kRowElems];
+    static_assert(sizeof(T) == 4, "values of two bytes are read in pieces");
 #pragma unroll
     for (int k = 0; k < kRowElems; ++k) {
-      q[k] = from_f32<T>(neg_inf());
-      const int c = k * lanes + lane;
-      if (c < len) q[k] = p[c];
+      const int c = at.index(k);
+      z[k] = __uint_as_float(fill);
+      if (c < at.len) z[k] = p[c];
     }
-#pragma unroll
-    for (int k = 0; k < kRowElems; ++k) z[k] = to_f32(q[k]);
   } else {
     constexpr int NV = kRowElems / VEC;
     uint4 q[NV];
-    const uint32_t low = neg_inf_bits<T>();
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (v * lanes + lane) * VEC;
-      q[v] = make_uint4(low, low, low, low);
-      if (c + VEC <= len) q[v] = *reinterpret_cast<const uint4*>(p + c);
+      const int c = at.index(v * VEC);
+      q[v] = make_uint4(fill, fill, fill, fill);
+      if (at.whole(c)) q[v] = *reinterpret_cast<const uint4*>(p + c);
     }
-    if (len % VEC != 0) {  // the piece that the end falls into
+    if (at.shift != 0 || at.len % VEC != 0) {
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const int c = (v * lanes + lane) * VEC;
-        if (c < len && c + VEC > len) {
+        const int c = at.index(v * VEC);
+        if (c + VEC > 0 && c < at.len && !at.whole(c)) {
           T e[VEC];
+          *reinterpret_cast<uint4*>(e) = q[v];
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            e[i] = from_f32<T>(neg_inf());
-            if (c + i < len) e[i] = p[c + i];
-          }
+          for (int i = 0; i < VEC; ++i)
+            if (at.has(c + i)) e[i] = p[c + i];
           q[v] = *reinterpret_cast<const uint4*>(e);
         }
       }
@@ -126,29 +150,83 @@ __device__ __forceinline__ void load_row(const T* __restrict__ p, int len, int l
   }
 }
 
-// Writes d[] to the same places, rounded once. The stretch begins on a 16-byte
-// boundary and its rows are whole pieces where VEC > 1.
-template <int VEC, typename T>
-__device__ __forceinline__ void store_row(T* __restrict__ p, int len, int lanes, int lane,
-                                          const float (&d)[kRowElems]) {
+// The same values one by one, for rows that lie differently to the 16-byte
+// boundaries than the result that `at` deals out.
+template <typename T, Mode M>
+__device__ __forceinline__ void load_row_single(const T* __restrict__ p, const Deal<T, M>& at,
+                                                float (&z)[kRowElems]) {
+  T q[kRowElems];
+#pragma unroll
+  for (int k = 0; k < kRowElems; ++k) {
+    const int c = at.index(k);
+    q[k] = from_f32<T>(0.0f);
+    if (at.has(c)) q[k] = p[c];
+  }
+#pragma unroll
+  for (int k = 0; k < kRowElems; ++k) z[k] = to_f32(q[k]);
+}
+
+// Writes d[] to the places of a lane's values, rounded once.
+template <typename T, Mode M>
+__device__ __forceinline__ void store_row(T* __restrict__ p, const Deal<T, M>& at, const float (&d)[kRowElems]) {
+  constexpr int VEC = Deal<T, M>::VEC;
   if constexpr (VEC == 1) {
 #pragma unroll
     for (int k = 0; k < kRowElems; ++k) {
-      const int c = k * lanes + lane;
-      if (c < len) p[c] = from_f32<T>(d[k]);
+      const int c = at.index(k);
+      if (c < at.len) p[c] = from_f32<T>(d[k]);
     }
   } else {
 #pragma unroll
     for (int v = 0; v < kRowElems / VEC; ++v) {
-      const int c = (v * lanes + lane) * VEC;
-      uint4 q;
-      T* e = reinterpret_cast<T*>(&q);
+      const int c = at.index(v * VEC);
+      T e[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) e[i] = from_f32<T>(d[v * VEC + i]);
-      if (c < len) *reinterpret_cast<uint4*>(p + c) = q;
+      if (at.whole(c)) {
+        *reinterpret_cast<uint4*>(p + c) = *reinterpret_cast<const uint4*>(e);
+      } else if (c + VEC > 0 && c < at.len) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (at.has(c + i)) p[c + i] = e[i];
+      }
     }
   }
 }
+
+// Counts of codes as floats, in two layouts: by code, and by code modulo 8 (values
+// that lie `lanes` pieces of 8 apart then lie side by side, at any shift).
+// `codes` is the codebook's size; both are padded to a multiple of 8.
+struct Counts {
+  const float* by_code;
+  const float* by_eight;
+  int64_t eights;  // codes / 8, rounded up
+  // Of the codes from c0 on, a multiple of 8.
+  __device__ __forceinline__ Counts from(int64_t c0) const { return Counts{by_code + c0, by_eight + c0 / 8, eights}; }
+  // Those of a lane's values k .. k + 3; 0 where it has none.
+  template <typename T, Mode M>
+  __device__ __forceinline__ void four(const Deal<T, M>& at, int k, float (&n)[4]) const {
+    const int c = at.index(k);
+    if constexpr (M == Mode::kWide) {
+      const float4 q = c < at.len ? *reinterpret_cast<const float4*>(by_code + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+      n[0] = q.x, n[1] = q.y, n[2] = q.z, n[3] = q.w;
+    } else if constexpr (M == Mode::kShifted) {
+      static_assert(Deal<T, M>::VEC == 8, "values of two bytes");
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // The same residue modulo 8 in every lane.
+        n[i] = 0.0f;
+        if (at.has(c + i)) n[i] = by_eight[((k % 8 + i - at.shift) & 7) * eights + ((c + i) >> 3)];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int ci = at.index(k + i);
+        n[i] = ci < at.len ? by_code[ci] : 0.0f;
+      }
+    }
+  }
+};
 
 // m: largest value (NaN aside), a: its first index, s: s' (NaN if the stretch
 // holds a NaN), w: t or u, n: n_a (u alone).
@@ -184,77 +262,51 @@ __device__ __forceinline__ RowStat shuffle_join(RowStat x, int offset, int width
   return join<kCounts>(x, y);
 }
 
-// Largest of a lane's values; NaN loses against any number.
-__device__ __forceinline__ float lane_max(const float (&z)[kRowElems]) {
-  float m[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) m[k] = fmaxf(fmaxf(z[k], z[k + 8]), fmaxf(z[k + 16], z[k + 24]));
-  return fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), fmaxf(fmaxf(m[4], m[5]), fmaxf(m[6], m[7])));
-}
-
-// Softmax sums of the values that WIDTH lanes hold (a stretch of len values, dealt
-// out to `lanes` lanes by load_row; the other lanes of the row, if any, make their
-// own). kCounts: n[] are the counts of a lane's own values, count_of(c) any one's.
-// The index in the result is the stretch's.
-template <int VEC, int WIDTH, bool kCounts, typename CountOf>
-__device__ __forceinline__ RowStat row_stat(const float (&z)[kRowElems], int len, int lanes, int lane,
-                                            const float* __restrict__ counts, CountOf&& count_of) {
-  RowStat r;
-  const float mine = lane_max(z);
-  r.m = mine;
-#pragma unroll
-  for (int o = WIDTH / 2; o > 0; o >>= 1) r.m = fmaxf(r.m, __shfl_xor_sync(kFullMask, r.m, o, WIDTH));
-  int at = kRowElems, same = 0;  // where the largest value is, how often
-  if (mine == r.m) {
-#pragma unroll
-    for (int k = kRowElems - 1; k >= 0; --k)
-      if (z[k] == r.m) at = k, ++same;
-  }
-  const uint32_t own = at < kRowElems ? (uint32_t)row_index<VEC>(lanes, lane, at) : 0x7fffffffu;
-  uint32_t a = own;
-#pragma unroll
-  for (int o = WIDTH / 2; o > 0; o >>= 1) a = min(a, __shfl_xor_sync(kFullMask, a, o, WIDTH));
-  r.a = min(a, (uint32_t)(len - 1));  // NaN alone: any
-  r.n = kCounts ? count_of((int)r.a) : 0.0f;
-  // The 1 of a itself is never added: it would swallow what s' is in a row with one certain code.
-  float s = (float)(own == a && at < kRowElems ? same - 1 : same), w = 0.0f;
-  constexpr int P = VEC == 1 ? 1 : 4;  // counts that one load brings
-#pragma unroll
-  for (int k0 = 0; k0 < kRowElems; k0 += P) {
-    float n[P];
-    if constexpr (kCounts) {
-      const int c = row_index<VEC>(lanes, lane, k0);
-      if constexpr (P == 4) {
-        const float4 q = c < len ? *reinterpret_cast<const float4*>(counts + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-        n[0] = q.x, n[1] = q.y, n[2] = q.z, n[3] = q.w;
-      } else {
-        n[0] = c < len ? counts[c] : 0.0f;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const float zk = z[k0 + i];
-      const float x = zk - r.m;
-      const float e = ex2_approx(x * kLog2e);
-      if (!(zk >= r.m)) s += e;  // a NaN is added
-      if constexpr (kCounts) {
-        w = fmaf(e, n[i] - r.n, w);  // 0 at a itself; its equals count in full
-      } else {
-        // x = -inf: e is 0, and so is its term (the bound is far below the range of exp).
-        const float t = max_nan(x, -200.0f);
-        if (!(zk >= r.m)) w = fmaf(e, t, w);
-      }
-    }
-  }
-#pragma unroll
-  for (int o = WIDTH / 2; o > 0; o >>= 1) {
-    s += __shfl_xor_sync(kFullMask, s, o, WIDTH);
-    w += __shfl_xor_sync(kFullMask, w, o, WIDTH);
-  }
-  r.s = s;
-  r.w = w;
+__device__ __forceinline__ float max3(float a, float b, float c) {  // NaN loses against any number
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Largest of a lane's values (NaN loses), by way of its eight runs of four.
+__device__ __forceinline__ float lane_max(const float (&z)[kRowElems], float (&four)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) four[j] = fmaxf(max3(z[4 * j], z[4 * j + 1], z[4 * j + 2]), z[4 * j + 3]);
+  return max3(max3(four[0], four[1], four[2]), max3(four[3], four[4], four[5]), fmaxf(four[6], four[7]));
+}
+__device__ __forceinline__ float lane_max(const float (&z)[kRowElems]) {
+  float four[8];
+  return lane_max(z, four);
+}
+// Smallest of a lane's values (NaN loses).
+__device__ __forceinline__ float lane_min(const float (&z)[kRowElems]) {
+  float m = min3(z[0], z[1], z[2]);
+#pragma unroll
+  for (int k = 3; k + 1 < kRowElems; k += 2) m = min3(m, z[k], z[k + 1]);
+  return fminf(m, z[kRowElems - 1]);
+}
+
+// exp of values relative to a row's m, as 2^y with y = z log2 e - M in one rounding,
+// M = m log2 e rounded. What that rounding left, d = m log2 e - M, is the same
+// factor 2^d on every value; it is taken out of the sums (`undo` = 2^-d). Where m is
+// far from 0 that factor leaves its range: `far` rows take z - m first.
+struct Base {
+  float m, neg_M, d, undo;
+  bool far;
+  __device__ __forceinline__ explicit Base(float m_) : m(m_) {
+    far = !(fabsf(m) <= 1024.0f);  // -inf and NaN too
+    neg_M = -__fmul_rn(m, kLog2e);
+    d = fmaf(m, kLog2e, neg_M);
+    undo = ex2_approx(-d);
+  }
+};
+constexpr float kLn2 = 0.6931471805599453f;
+// Below this z log2 e may be -inf, and its product with e = 0 NaN.
+constexpr float kLowest = -1e38f;
 
 // How the rows of a call are taken: `lanes` a row (kGroupMaxLanes or fewer: rows
 // side by side in a warp), else warps per stretch and stretches per row.
@@ -264,20 +316,23 @@ struct RowPlan {
 };
 // Stretches: as few as 8,192 values allow, more where that leaves fewer than two
 // blocks an SM, but none below 1,024 values (a warp's).
-inline RowPlan row_plan(int64_t rows, int64_t codes) {
+// Mode::kShifted needs up to 7 places more.
+inline RowPlan row_plan(int64_t rows, int64_t codes, bool shifted) {
   RowPlan p;
-  if (codes <= kGroupMaxCodes) {
+  const int64_t room = shifted ? 7 : 0;
+  if (codes + room <= kGroupMaxCodes) {
     p.lanes = 2;
-    while ((int64_t)p.lanes * kRowElems < codes) p.lanes *= 2;
+    while ((int64_t)p.lanes * kRowElems < codes + room) p.lanes *= 2;
     return p;
   }
   constexpr int64_t kFill = 2 * 148;
-  int64_t parts = (codes + kBlockMaxCodes - 1) / kBlockMaxCodes;
+  const int64_t most = kBlockMaxCodes - (shifted ? 8 : 0);
+  int64_t parts = (codes + most - 1) / most;
   if (rows * parts < kFill) parts = std::max(parts, std::min((codes + 1023) / 1024, (kFill + rows - 1) / rows));
   const int64_t len = ((codes + parts - 1) / parts + 7) / 8 * 8;  // 16-byte boundaries of every type
   p.part_len = (int)len;
   p.parts = (int)((codes + len - 1) / len);
-  while (p.warps * 32 * kRowElems < len) p.warps *= 2;
+  while (p.warps * 32 * kRowElems < len + room) p.warps *= 2;
   return p;
 }
 
@@ -296,16 +351,42 @@ inline void with_warps(int warps, Fn&& fn) {
   else if (warps == 4) fn(std::integral_constant<int, 4>{});
   else fn(std::integral_constant<int, 8>{});
 }
-// Calls fn(T{}, integral constant VEC).
+template <Mode M>
+using ModeOf = std::integral_constant<Mode, M>;
+// How the rows at p lie: pieces of 16 bytes where all begin on such a boundary;
+// values of two bytes in shifted pieces elsewhere, of four one by one (a warp's 128
+// bytes a load already).
+inline Mode row_mode(int32_t dtype, const void* p, int64_t stride) {
+  if (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * dtype_bytes(dtype) % 16 == 0) return Mode::kWide;
+  return dtype == GSB_DTYPE_F32 ? Mode::kSingle : Mode::kShifted;
+}
+// Calls fn(T{}, ModeOf<>{}).
 template <typename Fn>
-inline void with_rows(int32_t dtype, bool wide, Fn&& fn) {
+inline void with_rows(int32_t dtype, Mode mode, Fn&& fn) {
   with_dtype(dtype, [&](auto t) {
-    if (wide) fn(t, std::integral_constant<int, wide_of<decltype(t)>()>{});
-    else fn(t, std::integral_constant<int, 1>{});
+    if (mode == Mode::kWide) fn(t, ModeOf<Mode::kWide>{});
+    else if constexpr (sizeof(t) == 4) fn(t, ModeOf<Mode::kSingle>{});
+    else fn(t, ModeOf<Mode::kShifted>{});
   });
 }
-inline bool rows_wide(int32_t dtype, const void* p, int64_t stride) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * dtype_bytes(dtype) % 16 == 0;
+// The backward's, by the result's rows; the third argument says whether the logits'
+// rows lie as the result's do.
+template <typename Fn>
+inline void with_row_pairs(int32_t dtype, const void* in, int64_t in_stride, const void* out, int64_t out_stride,
+                           Fn&& fn) {
+  const int64_t size = dtype_bytes(dtype);
+  const bool same = (reinterpret_cast<uintptr_t>(in) - reinterpret_cast<uintptr_t>(out)) % 16 == 0 &&
+                    (in_stride - out_stride) * size % 16 == 0;
+  Mode mode = row_mode(dtype, out, out_stride);
+  if (!same) mode = dtype == GSB_DTYPE_F32 ? Mode::kSingle : Mode::kShifted;
+  with_rows(dtype, mode, [&](auto t, auto m) {
+    if constexpr (decltype(m)::value == Mode::kShifted) {
+      if (same) fn(t, m, std::true_type{});
+      else fn(t, m, std::false_type{});
+    } else {
+      fn(t, m, std::true_type{});
+    }
+  });
 }
 
 inline int check_rows(int32_t dtype, int64_t rows, int64_t codes, int64_t stride, int32_t code_bytes) {

@@ -17,6 +17,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAEvent.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <array>
@@ -982,6 +983,142 @@ Tensor op_code_balance_bwd(const Tensor& g_loss, const Tensor& logits, const Ten
   return dz;
 }
 
+// Autograd of the three operators, in C++ so that a backward needs no interpreter
+// on the engine's device thread. Gradients of gradients are refused when taken.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  auto refuse = std::make_shared<torch::autograd::DelayedError>(
+      "gsplat_b200: the codebook operators are differentiable once", grads.size());
+  variable_list in;
+  for (const Tensor& g : grads) in.push_back(g.defined() ? g.detach().requires_grad_(true) : g);
+  return (*refuse)(std::move(in));
+}
+std::optional<Tensor> maybe(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+
+struct LookupFn : torch::autograd::Function<LookupFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& codebook, const Tensor& codes,
+                        const std::optional<Tensor>& weights, double scale, at::ScalarType out_dtype) {
+    ctx->save_for_backward({codebook, codes, weights.value_or(Tensor())});
+    ctx->saved_data["scale"] = scale;
+    return op_codebook_fwd(codebook, codes, weights, scale, out_dtype);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const variable_list t = ctx->get_saved_variables();
+    auto [g_codebook, g_weights] =
+        op_codebook_bwd(g[0], t[0], t[1], maybe(t[2]), ctx->saved_data["scale"].toDouble(),
+                        ctx->needs_input_grad(0), t[2].defined() && ctx->needs_input_grad(2));
+    return once({g_codebook, Tensor(), g_weights, Tensor(), Tensor()});
+  }
+};
+
+struct LogProbsFn : torch::autograd::Function<LogProbsFn> {
+  // -> entropy, top_log_probs, top_codes, and log_probs where there are codes
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const std::optional<Tensor>& codes,
+                               int64_t top_k) {
+    auto [lp, ent, tl, tc, stats] = op_code_log_probs_fwd(logits, codes, top_k, true);
+    ctx->save_for_backward({logits, codes.value_or(Tensor()), tc, stats});
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({tc});
+    if (lp.defined()) return {ent, tl, tc, lp};
+    return {ent, tl, tc};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const Tensor g_lp = g.size() > 3 ? g[3] : Tensor();
+    if (!g[0].defined() && !g[1].defined() && !g_lp.defined()) return {Tensor(), Tensor(), Tensor()};
+    const variable_list t = ctx->get_saved_variables();
+    const Tensor dz = op_code_log_probs_bwd(maybe(g_lp), maybe(g[0]), maybe(g[1]), t[0], maybe(t[1]), t[2], t[3]);
+    return once({dz, Tensor(), Tensor()});
+  }
+};
+
+struct BalanceFn : torch::autograd::Function<BalanceFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& codes) {
+    auto [loss, counts, stats, state] = op_code_balance_fwd(logits, codes, true);
+    ctx->save_for_backward({logits, stats, state});
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({counts});
+    return {loss, counts};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    if (!g[0].defined()) return {Tensor(), Tensor()};
+    const variable_list t = ctx->get_saved_variables();
+    return once({op_code_balance_bwd(g[0], t[0], t[1], t[2]), Tensor()});
+  }
+};
+
+// Argument checks of the public functions, made before anything needs a GPU. Shapes
+// that are not these are refused by the ops themselves.
+void check_code_args(const Tensor& t, const char* name, const Tensor& codes) {
+  const auto dt = t.scalar_type();
+  if (dt != at::kFloat && dt != at::kBFloat16 && dt != at::kHalf)
+    value_error(std::string(name) + " must be float32, bfloat16 or float16");
+  if (codes.defined() && codes.scalar_type() != at::kInt && codes.scalar_type() != at::kLong)
+    value_error("codes must be int32 or int64");
+  if (!t.is_cuda() || (codes.defined() && codes.device() != t.device()))
+    value_error(std::string(name) + " and codes must be on the same CUDA device");
+}
+bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+Tensor codebook_lookup(const Tensor& codebook, const Tensor& codes, const std::optional<Tensor>& weights, double scale,
+                       const std::optional<at::ScalarType>& out_dtype) {
+  if (codebook.dim() < 1 || codebook.numel() == 0)
+    value_error("codebook must have shape [C, ...] with at least one row and value");
+  const Tensor w = weights.value_or(Tensor());
+  if (w.defined()) {
+    if (codes.dim() < 1 || w.sizes() != codes.sizes() || codes.size(-1) < 1)
+      value_error("weights must have the shape [..., J] of codes");
+    if (w.scalar_type() != at::kFloat) value_error("weights must be float32");
+    if (w.device() != codebook.device()) value_error("weights and codebook must be on the same CUDA device");
+  }
+  const at::ScalarType out = out_dtype.value_or(codebook.scalar_type());
+  if (out != codebook.scalar_type() && out != at::kFloat) value_error("out_dtype must be the codebook's or float32");
+  check_code_args(codebook, "codebook", codes);
+  if (at::GradMode::is_enabled() && (codebook.requires_grad() || wants_grad(w)))
+    return LookupFn::apply(codebook, codes, weights, scale, out);
+  return op_codebook_fwd(codebook, codes, weights, scale, out);
+}
+
+// -> log_probs (None without codes), entropy, top_log_probs, top_codes
+std::tuple<std::optional<Tensor>, Tensor, Tensor, Tensor> code_log_probs(const Tensor& logits,
+                                                                         const std::optional<Tensor>& codes,
+                                                                         int64_t top_k) {
+  if (logits.dim() < 1 || logits.size(-1) < 1)
+    value_error("logits must have shape [..., C] with at least one code");
+  const Tensor c = codes.value_or(Tensor());
+  if (c.defined() && c.sizes() != logits.sizes().slice(0, logits.dim() - 1))
+    value_error("codes must have the shape [...] of logits [..., C]");
+  if (top_k < 0 || top_k > std::min<int64_t>(GSB_CODE_MAX_TOP, logits.size(-1)))
+    value_error("top_k must be between 0 and min(" + std::to_string(GSB_CODE_MAX_TOP) + ", C); got " +
+                std::to_string(top_k));
+  check_code_args(logits, "logits", c);
+  if (at::GradMode::is_enabled() && logits.requires_grad()) {
+    const variable_list r = LogProbsFn::apply(logits, codes, top_k);
+    return {r.size() > 3 ? std::optional<Tensor>(r[3]) : std::nullopt, r[0], r[1], r[2]};
+  }
+  auto [lp, ent, tl, tc, stats] = op_code_log_probs_fwd(logits, codes, top_k, false);
+  return {maybe(lp), ent, tl, tc};
+}
+
+std::tuple<Tensor, Tensor> code_balance_loss(const Tensor& logits, const Tensor& codes) {
+  if (logits.dim() < 1 || logits.size(-1) < 1)
+    value_error("logits must have shape [..., C] with at least one code");
+  const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+  const auto given = codes.sizes();
+  const bool flat = given == lead;
+  const bool bag = codes.dim() == logits.dim() && given.slice(0, codes.dim() - 1) == lead && codes.size(-1) >= 1;
+  if (!flat && !bag) value_error("codes must have the shape [...] or [..., J] of logits [..., C]");
+  check_code_args(logits, "logits", codes);
+  if (at::GradMode::is_enabled() && logits.requires_grad()) {
+    const variable_list r = BalanceFn::apply(logits, codes);
+    return {r[0], r[1]};
+  }
+  auto [loss, counts, stats, state] = op_code_balance_fwd(logits, codes, false);
+  return {loss, counts};
+}
+
 void check_device_errors() {
   errors().check_all(nullptr);
   mapped_status().check_all();
@@ -1066,6 +1203,9 @@ TORCH_LIBRARY_IMPL(gsplat_b200, CUDA, m) {
 PYBIND11_MODULE(_gsb_host, m) {
   m.doc() = "Native host runtime of the B200 rasterizer autograd path (drives the C ABI).";
   m.def("check_device_errors", &check_device_errors);
+  m.def("codebook_lookup", &codebook_lookup);
+  m.def("code_log_probs", &code_log_probs);
+  m.def("code_balance_loss", &code_balance_loss);
   m.def("set_phase_timing", &set_phase_timing);
   m.def("take_phase_times", &take_phase_times);
 }
