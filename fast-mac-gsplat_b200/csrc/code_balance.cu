@@ -13,6 +13,10 @@ constexpr int kGroupThreads = 256;
 constexpr int kCountBlocks = 2 * 148;
 constexpr int kCountSharedCodes = 8192;  // counts that a block keeps in shared memory
 constexpr int kCountFew = 8192;          // slots that one block counts alone
+// Blocks an SM. Short rows wait for memory (65,536 x 1,000 fp32: 62 us with 6, 70 with
+// 4); long ones want registers (16,384 x 16,383 fp16, with the backward: 583 and 550 us).
+constexpr int kBalanceBlocksShort = 6;
+constexpr int kBalanceBlocksLong = 4;
 constexpr int kBalanceSums = 32 * 148;   // sums over rows, at most
 constexpr int kStateHead = 8;  // floats before the counts in `state`; [0]: C / (rows with a code x codes counted)
 
@@ -126,32 +130,27 @@ __device__ __forceinline__ float finish(RowStat r, bool valid, float4* stats) {
 
 // parts > 1: a part's sums go to `stat` and `stat_a` for k_balance_join.
 template <typename T, int L>
-__global__ void __launch_bounds__(kTileWarps * 32)
+__global__ void __launch_bounds__(kTileWarps * 32, L < 32 ? kBalanceBlocksShort : kBalanceBlocksLong)
     k_balance(TileRows<T> t, int bag, Codes codes, Counts counts, float4* __restrict__ stats,
               float4* __restrict__ stat, uint32_t* __restrict__ stat_a, double* __restrict__ sums) {
   pdl_wait();
   pdl_trigger();
-  __shared__ uint4 s_buf[kTileWarps][kTileStages * kTilePieces * 32];
+  extern __shared__ uint4 s_buf[];
   const int warp = threadIdx.x / 32, lane32 = threadIdx.x % 32, lane = lane32 % L;
-  int64_t next_code = -1, code = -1;  // one of the row's; a lane takes more only where there are more than lanes
+  int64_t code = -1;  // one of the row's; a lane takes more only where there are more than lanes
   RowStat row;
   double sum = 0.0;
   walk_tiles<T, L>(
-      t, s_buf[warp], lane32,
-      [&](const TilePlace<T, L>& next) {
-        next_code = lane < bag ? codes.at(next.row * bag + lane) : -1;
+      t, s_buf + warp * kTilePieces * 32, lane32, false,
+      [&](const TilePlace<T, L>& place) { code = lane < bag ? codes.at(place.row * bag + lane) : -1; },
+      [&](const TilePlace<T, L>& now, int slice, const Slice<T, L>& at, const LaneBuf& buf, auto&& refill) {
+        float second;
+        RowStat r = lane_sums<true>(buf, at, counts.from(now.c0), second, [](int, float) {}, refill);
+        if (L == 32 && r.a != 0xffffffffu) r.a += (uint32_t)now.c0;
+        row = slice == 0 ? r : join<true>(row, r);
       },
-      [&] { code = next_code; },
-      [&](const TilePlace<T, L>& now, uint4* buf) {
-        RowStat r = lane_sums<true>(buf, now.values(lane32), counts.from(now.c0));
-        if (L == 32) {
-          if (r.a != 0xffffffffu) r.a += (uint32_t)now.c0;
-          row = now.slice == 0 ? r : join<true>(row, r);
-          if (now.slice + 1 < now.slices) return;
-          r = row;
-        }
-#pragma unroll
-        for (int d = L / 2; d > 0; d >>= 1) r = shuffle_join<true>(r, d, L);
+      [&](const TilePlace<T, L>& now, const Slice<T, L>&, const LaneBuf&) {
+        const RowStat r = join_lanes<true, L>(row);
         int valid = code >= 0 && code < t.codes;
         for (int j = lane + L; j < bag; j += L) {
           const int64_t c = codes.at(now.row * bag + j);
@@ -174,6 +173,10 @@ __global__ void __launch_bounds__(kTileWarps * 32)
     if (lane32 == 0) sums[blockIdx.x * kTileWarps + warp] = sum;
   }
 }
+TilePlan balance_plan(int64_t rows, int64_t codes, int size, bool shifted) {
+  return tile_plan(std::max<int64_t>(rows, 1), codes, size, shifted, 1 << 20, kBalanceBlocksLong,
+                   kBalanceBlocksShort);
+}
 
 // A warp per row joins its stretches' sums.
 __global__ void __launch_bounds__(128)
@@ -191,8 +194,7 @@ __global__ void __launch_bounds__(128)
       const float4 v = stat[row * parts + i];
       r = join<true>(r, RowStat{v.x, v.y, v.z, v.w, stat_a[row * parts + i]});
     }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) r = shuffle_join<true>(r, d, 32);
+    r = join_lanes<true, 32>(r);
     const bool valid = any_code<32>(codes, row, bag, C, lane);
     if (lane == 0) sum += (double)finish(r, valid, stats ? stats + row : nullptr);
   }
@@ -328,7 +330,7 @@ extern "C" size_t gsb_code_balance_workspace_size(int64_t rows, int64_t codebook
   for (int size = 2; size <= 4; size += 2) {
     for (int shifted = 0; shifted < 2; ++shifted) {
       Carver c(nullptr);
-      carve(c, rows, tile_plan(std::max<int64_t>(rows, 1), codebook_rows, size, shifted));
+      carve(c, rows, balance_plan(rows, codebook_rows, size, shifted));
       need = std::max(need, c.off);
     }
   }
@@ -347,8 +349,8 @@ extern "C" int gsb_code_balance_forward(int32_t dtype, int64_t rows, int64_t cod
   if (!workspace || workspace_bytes < gsb_code_balance_workspace_size(rows, codebook_rows)) return GSB_ERR_WORKSPACE;
   if (rows == 1) logits_stride = 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const TilePlan plan = tile_plan(std::max<int64_t>(rows, 1), codebook_rows, dtype_bytes(dtype),
-                                  rows_shifted(dtype_bytes(dtype), logits, logits_stride));
+  const TilePlan plan = balance_plan(rows, codebook_rows, dtype_bytes(dtype),
+                                     rows_shifted(dtype_bytes(dtype), logits, logits_stride));
   Carver ws(workspace);
   const BalanceScratch b = carve(ws, rows, plan);
   const Codes cd{codes, code_bytes == 8};
@@ -381,10 +383,11 @@ extern "C" int gsb_code_balance_forward(int32_t dtype, int64_t rows, int64_t cod
       using T = decltype(tag);
       const int64_t items = plan.items(rows);
       const TileRows<T> t{(const T*)logits, logits_stride, rows, codebook_rows, plan.part_len, items, plan.parts};
-      const int blocks = tile_blocks(items);
+      const int blocks = plan.blocks(rows);
       n_sums = blocks * kTileWarps;
       with_tile_lanes(plan.lanes, [&](auto l) {
-        launch_pdl(k_balance<T, decltype(l)::value>, blocks, kTileWarps * 32, 0, s, t, bag, cd, counts_f32,
+        launch_pdl(k_balance<T, decltype(l)::value>, blocks, kTileWarps * 32,
+                   kTileWarps * kTilePieces * 32 * sizeof(uint4), s, t, bag, cd, counts_f32,
                    (float4*)stats, b.stat, b.stat_a, b.sums);
       });
     });

@@ -46,19 +46,18 @@ __device__ __forceinline__ int64_t given_code(const LogProbsOut& o, const Codes&
 // one: every lane has its own largest, taken out of the buffer; the row's largest of
 // those is next, and its lane looks for another.
 template <typename T, int L>
-__device__ __forceinline__ void pick_alternatives(uint4* buf, int lane, const TilePlace<T, L>& now,
+__device__ __forceinline__ void pick_alternatives(const LaneBuf& buf, int lane, const TilePlace<T, L>& now,
                                                   const Slice<T, L>& at, const RowStat& own, const RowResult& q,
                                                   const LogProbsOut& o, int top_k) {
   constexpr int VEC = wide_of<T>();
   uint64_t best = own.a == 0xffffffffu ? 0 : order_key(own.m, own.a);
   int nan_from = 0;
   // What is out is NaN from here on.
-  auto take = [&](int c) {
-    const int k = c - at.first;  // pieces lie L VEC apart
-    reinterpret_cast<T*>(buf + k / (L * VEC) * 32)[k % (L * VEC)] = from_f32<T>(quiet_nan());
-  };
   if (at.ragged()) fill_ragged(buf, at, quiet_nan());
-  if (best != 0) take((int)own.a);
+  if (best != 0) {
+    const int k = (int)own.a - at.first;  // pieces lie L VEC apart
+    reinterpret_cast<T*>(&buf[k / (L * VEC)])[k % (L * VEC)] = from_f32<T>(quiet_nan());
+  }
   for (int j = 0;; ++j) {
     uint64_t row_best = best;
 #pragma unroll
@@ -79,26 +78,14 @@ __device__ __forceinline__ void pick_alternatives(uint4* buf, int lane, const Ti
     }
     if (j + 1 == top_k) break;
     if (best == row_best && best != 0) {
-      float top = quiet_nan();
-      int top_v = 0;
-#pragma unroll
-      for (int v = 0; v < kTilePieces; ++v) {
-        if (v < at.n) {
-          float hi, lo;
-          piece_range(buf[v * 32], T{}, hi, lo);
-          if (hi == hi && !(hi <= top)) top = hi, top_v = v;  // the first of equal ones
-        }
-      }
+      const LaneTop top = lane_top(buf, at, [](int, float) {});
       best = 0;
-      if (top == top) {
-        float f[VEC];
-        unpack<T>(buf[top_v * 32], f);
-        int c = 0;
-#pragma unroll
-        for (int i = VEC - 1; i >= 0; --i)
-          if (f[i] == top) c = at.at(top_v) + i;
-        best = order_key(top, (uint32_t)c);
-        take(c);
+      if (top.m == top.m) {
+        int v, i;
+        float rest;
+        find_value<T>(buf, top.group, top.m, &v, &i, &rest);
+        best = order_key(top.m, (uint32_t)(at.at(v) + i));
+        reinterpret_cast<T*>(&buf[v])[i] = from_f32<T>(quiet_nan());
       }
     }
   }
@@ -106,57 +93,101 @@ __device__ __forceinline__ void pick_alternatives(uint4* buf, int lane, const Ti
 
 // The k largest keys of a part of a row, to put(rank, key). k lanes hold a value of
 // at least the k-th largest of the lanes' maxima, so none of the k largest is below
-// that; the slices of lanes that reach it are read again (they come from L2) and the
-// few values that do are listed and ranked against one another. Many equal values can
-// overrun the list: then the part is searched once for each key.
+// that. As a rule (4 alternatives: four rows in five) no lane's second value reaches
+// it, and the lanes' maxima are all there is to rank. Else those lanes read the groups
+// of pieces that reach it again (they come from L2), and the few values that do are
+// listed and ranked against one another. Many equal values can overrun the list: then
+// the part is searched once for each key.
 constexpr int kTopList = 128;
+// 128 registers a thread: with 80, for 6 blocks, the same kernels took 653 / 169 / 185 us
+// where they take 615 / 164 / 170 (65,536 x 4,096 fp32, 2,047 x 50,001 fp16 and 2^20 x 64
+// bf16, forward and backward).
+constexpr int kLogProbsBlocksSM = 4;
+constexpr int kTopSlices = 2;  // of a part with more than one alternative
+constexpr int kTopGroups = kTopSlices * kTilePieces / kTileGroup;
+struct TopSmem {
+  float top[kTopGroups][32];
+  uint64_t list[kTopList];
+  int count;
+};
 template <typename T, typename Put>
-__device__ __forceinline__ void list_alternatives(const TilePlace<T, 32>& now, int lane, float lane_best, int k,
-                                                  const float (*top)[32], uint64_t* list, int* count, Put&& put) {
+__device__ __forceinline__ void list_alternatives(const TilePlace<T, 32>& now, int lane, const RowStat& own,
+                                                  float second, int k, TopSmem& sm, Put&& put) {
   constexpr int VEC = wide_of<T>();
-  uint32_t left = order_bits(lane_best), bound = 0;
+  constexpr int kGroups = kTilePieces / kTileGroup;  // of a slice
+  uint32_t left = order_bits(own.m), bound = 0;
   for (int j = 0; j < k; ++j) {
     bound = __reduce_max_sync(kFullMask, left);
     const uint32_t who = __ballot_sync(kFullMask, left == bound);
     if (lane == __ffs(who) - 1) left = 0;
   }
   const float least = key_value((uint64_t)bound << 32);
-  if (lane == 0) *count = 0;
+  const bool again = second >= least;
+  const uint64_t own_key = order_key(own.m, own.a);
+  const bool single = own.m >= least && own.a != 0xffffffffu;  // a lane without a value has m = -inf
+  if (!__any_sync(kFullMask, again)) {
+    const uint32_t who = __ballot_sync(kFullMask, single);
+    if (__popc(who) >= k) {
+      int rank = 0;
+      for (uint32_t w = who; w != 0; w &= w - 1) rank += __shfl_sync(kFullMask, own_key, __ffs(w) - 1) > own_key;
+      if (single && rank < k) put(rank, own_key);
+      return;
+    }
+  }
+  if (lane == 0) sm.count = 0;
   __syncwarp();
-  for (int j = 0; j < now.slices; ++j) {
-    if (!(top[j][lane] >= least)) continue;
-    const Slice<T, 32> at(now.len, now.shift, j, lane);
-    for (int v = 0; v < kTilePieces; ++v) {
-      const int c = at.at(v);
-      if (c >= at.len) break;
-      float f[VEC];
+  uint32_t mine = 0;  // the lane's groups that reach it
+  if (again) {
+#pragma unroll
+    for (int g = 0; g < kTopGroups; ++g)
+      if (g < now.slices * kGroups && sm.top[g][lane] >= least) mine |= 1u << g;
+  } else if (single) {
+    const int to = atomicAdd(&sm.count, 1);
+    if (to < kTopList) sm.list[to] = own_key;
+  }
+  for (; mine != 0; mine &= mine - 1) {
+    const int g = __ffs(mine) - 1;
+    const Slice<T, 32> at(now.len, now.shift, g / kGroups, lane);
+    const int v0 = g % kGroups * kTileGroup;
+    uint4 q[kTileGroup];
+#pragma unroll
+    for (int v = 0; v < kTileGroup; ++v) {
+      const int c = at.at(v0 + v);
+      T e[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) e[i] = from_f32<T>(quiet_nan());
+      q[v] = *reinterpret_cast<const uint4*>(e);
       if (c >= 0 && c + VEC <= at.len) {
-        unpack<T>(*reinterpret_cast<const uint4*>(now.p + c), f);
-      } else {
+        q[v] = *reinterpret_cast<const uint4*>(now.p + c);
+      } else if (c < at.len && c + VEC > 0) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) f[i] = at.has(c + i) ? to_f32(now.p[c + i]) : quiet_nan();
+        for (int i = 0; i < VEC; ++i)
+          if (at.has(c + i)) e[i] = now.p[c + i];
+        q[v] = *reinterpret_cast<const uint4*>(e);
       }
-      float hi = f[0];
+    }
 #pragma unroll
-      for (int i = 1; i < VEC; ++i) hi = fmaxf(hi, f[i]);
-      if (hi >= least) {
+    for (int v = 0; v < kTileGroup; ++v) {
+      if (Range<T>(q[v]).top() >= least) {
+        float f[VEC];
+        unpack<T>(q[v], f);
+#pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          const float z = at.has(c + i) ? to_f32(now.p[c + i]) : quiet_nan();
-          if (z >= least) {
-            const int to = atomicAdd(count, 1);
-            if (to < kTopList) list[to] = order_key(z, (uint32_t)(now.c0 + c + i));
+          if (f[i] >= least) {
+            const int to = atomicAdd(&sm.count, 1);
+            if (to < kTopList) sm.list[to] = order_key(f[i], (uint32_t)(now.c0 + at.at(v0 + v) + i));
           }
         }
       }
     }
   }
   __syncwarp();
-  const int n = *count;
+  const int n = sm.count;
   if (n >= k && n <= kTopList) {
     for (int i = lane; i < n; i += 32) {
-      const uint64_t key = list[i];
+      const uint64_t key = sm.list[i];
       int rank = 0;
-      for (int j = 0; j < n; ++j) rank += list[j] > key;
+      for (int j = 0; j < n; ++j) rank += sm.list[j] > key;
       if (rank < k) put(rank, key);
     }
   } else {
@@ -181,46 +212,46 @@ __device__ __forceinline__ void list_alternatives(const TilePlace<T, 32>& now, i
 
 // parts > 1: a part's sums and keys go to `stat` and `keys` for k_log_probs_join.
 template <typename T, int L>
-__global__ void __launch_bounds__(kTileWarps * 32)
+__global__ void __launch_bounds__(kTileWarps * 32, kLogProbsBlocksSM)
     k_log_probs(TileRows<T> t, Codes codes, int top_k, LogProbsOut o, float4* __restrict__ stat,
                 uint64_t* __restrict__ keys, uint32_t* status) {
   pdl_wait();
   pdl_trigger();
-  __shared__ uint4 s_buf[kTileWarps][kTileStages * kTilePieces * 32];
-  __shared__ float s_top[L == 32 ? kTileWarps : 1][kTileSlices][32];
-  __shared__ uint64_t s_list[L == 32 ? kTileWarps : 1][kTopList];
-  __shared__ int s_count[kTileWarps];
+  extern __shared__ uint4 s_buf[];  // the warps' buffers, then (L = 32, top_k > 1) a TopSmem each
   const int warp = threadIdx.x / 32, lane32 = threadIdx.x % 32, lane = lane32 % L;
-  int64_t next_code = -1, code = -1;
+  TopSmem* tops = reinterpret_cast<TopSmem*>(s_buf + kTileWarps * kTilePieces * 32) + warp;
+  int64_t code = -1;
   float zc = 0.0f;
   const bool given = o.log_probs != nullptr && (L < 32 || t.parts == 1);
   RowStat sums;
+  float second = 0.0f;
   walk_tiles<T, L>(
-      t, s_buf[warp], lane32,
-      [&](const TilePlace<T, L>& next) {
-        if (given) next_code = codes.at(next.row);
+      t, s_buf + warp * kTilePieces * 32, lane32, L < 32 && top_k > 1,
+      [&](const TilePlace<T, L>& place) {
+        if (given) code = codes.at(place.row);
       },
-      [&] { code = next_code; },
-      [&](const TilePlace<T, L>& now, uint4* buf) {
-        if (now.slice == 0) {
+      [&](const TilePlace<T, L>& now, int slice, const Slice<T, L>& at, const LaneBuf& buf, auto&& refill) {
+        if (slice == 0) {
           if (code >= t.codes) {
             if (now.on && lane == 0) bad_code(status, kSiteCode);
             code = -1;
           }
           zc = code >= 0 ? to_f32(now.p[code]) : 0.0f;
         }
-        const Slice<T, L> at = now.values(lane32);
-        RowStat r = lane_sums<false>(buf, at, Counts{});
-        const RowStat own = r;
-        if (L == 32) {
-          if (top_k > 1) s_top[L == 32 ? warp : 0][now.slice][lane32] = r.m;
-          if (r.a != 0xffffffffu) r.a += (uint32_t)now.c0;
-          sums = now.slice == 0 ? r : join<false>(sums, r);
-          if (now.slice + 1 < now.slices) return;
-          r = sums;
-        }
-#pragma unroll
-        for (int d = L / 2; d > 0; d >>= 1) r = shuffle_join<false>(r, d, L);
+        float next_best;
+        RowStat r = lane_sums<false>(
+            buf, at, Counts{}, next_best,
+            [&](int v0, float top) {
+              if (L == 32 && top_k > 1)
+                tops->top[slice * (kTilePieces / kTileGroup) + v0 / kTileGroup][lane32] = top;
+            },
+            refill);
+        if (L == 32 && r.a != 0xffffffffu) r.a += (uint32_t)now.c0;
+        second = slice == 0 ? next_best : fmaxf(fmaxf(second, next_best), fminf(sums.m, r.m));
+        sums = slice == 0 ? r : join<false>(sums, r);
+      },
+      [&](const TilePlace<T, L>& now, const Slice<T, L>& at, const LaneBuf& buf) {
+        RowStat r = join_lanes<false, L>(sums);
         if (r.a == 0xffffffffu) r.a = (uint32_t)now.c0;  // NaN alone
         if (L < 32 || t.parts == 1) {
           const RowResult q = finish(r);
@@ -233,13 +264,12 @@ __global__ void __launch_bounds__(kTileWarps * 32)
           }
           if (top_k > 1) {
             if constexpr (L < 32)
-              pick_alternatives<T, L>(buf, lane, now, at, own, q, o, top_k);
+              pick_alternatives<T, L>(buf, lane, now, at, sums, q, o, top_k);
             else
-              list_alternatives(now, lane32, sums.m, top_k, s_top[warp], s_list[warp], &s_count[warp],
-                                [&](int j, uint64_t key) {
-                                  o.top_codes[now.row * top_k + j] = (int32_t)key_index(key);
-                                  o.top_log_probs[now.row * top_k + j] = q.log_p(key_value(key));
-                                });
+              list_alternatives(now, lane32, sums, second, top_k, *tops, [&](int j, uint64_t key) {
+                o.top_codes[now.row * top_k + j] = (int32_t)key_index(key);
+                o.top_log_probs[now.row * top_k + j] = q.log_p(key_value(key));
+              });
           }
         } else if constexpr (L == 32) {
           if (lane32 == 0) stat[now.item] = make_float4(r.m, r.s, r.w, __uint_as_float(r.a));
@@ -247,12 +277,17 @@ __global__ void __launch_bounds__(kTileWarps * 32)
           if (top_k == 1 && lane32 == 0) to[0] = order_key(r.m, r.a);
           if (top_k > 1) {
             const int k = min(top_k, now.len);
-            list_alternatives(now, lane32, sums.m, k, s_top[warp], s_list[warp], &s_count[warp],
-                              [&](int j, uint64_t key) { to[j] = key; });
+            list_alternatives(now, lane32, sums, second, k, *tops, [&](int j, uint64_t key) { to[j] = key; });
             for (int j = k + lane32; j < top_k; j += 32) to[j] = 0;  // a short last part
           }
         }
       });
+}
+
+// Parts of a call with more than one alternative have kTopSlices slices at most.
+TilePlan log_probs_plan(int64_t rows, int64_t codes, int size, bool shifted, int top_k) {
+  return tile_plan(rows, codes, size, shifted, top_k > 1 ? kTopSlices : 1 << 20, kLogProbsBlocksSM,
+                   kLogProbsBlocksSM);
 }
 
 // One warp per row joins its stretches' sums and picks the largest keys.
@@ -276,8 +311,7 @@ __global__ void __launch_bounds__(128)
   // A lane without a stretch adds nothing: -inf at an index behind all.
   RowStat r{neg_inf(), 0.0f, 0.0f, 0.0f, 0xffffffffu};
   for (int i = lane; i < parts; i += 32) r = join<false>(r, stat_at(i));
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) r = shuffle_join<false>(r, d, 32);
+  r = join_lanes<false, 32>(r);
   const RowResult q = finish(r);
   if (lane == 0) write_row(o, row, r, q, code, code >= 0, zc);
   const uint64_t* ks = keys + row * parts * top_k;
@@ -442,7 +476,7 @@ extern "C" size_t gsb_code_log_probs_workspace_size(int64_t rows, int64_t codebo
   for (int size = 2; size <= 4; size += 2) {
     for (int shifted = 0; shifted < 2; ++shifted) {
       Carver c(nullptr);
-      carve(c, rows, tile_plan(rows, codebook_rows, size, shifted), top_k);
+      carve(c, rows, log_probs_plan(rows, codebook_rows, size, shifted, top_k), top_k);
       need = std::max(need, c.off);
     }
   }
@@ -463,8 +497,8 @@ extern "C" int gsb_code_log_probs_forward(int32_t dtype, int64_t rows, int64_t c
   const size_t need = gsb_code_log_probs_workspace_size(rows, codebook_rows, top_k);
   if (need > 0 && (!workspace || workspace_bytes < need)) return GSB_ERR_WORKSPACE;
   if (rows == 1) logits_stride = 0;
-  const TilePlan plan = tile_plan(rows, codebook_rows, dtype_bytes(dtype),
-                                  rows_shifted(dtype_bytes(dtype), logits, logits_stride));
+  const TilePlan plan = log_probs_plan(rows, codebook_rows, dtype_bytes(dtype),
+                                       rows_shifted(dtype_bytes(dtype), logits, logits_stride), top_k);
   Carver ws(workspace);
   const LogProbsScratch b = carve(ws, rows, plan, top_k);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -474,8 +508,10 @@ extern "C" int gsb_code_log_probs_forward(int32_t dtype, int64_t rows, int64_t c
     using T = decltype(tag);
     const int64_t items = plan.items(rows);
     const TileRows<T> t{(const T*)logits, logits_stride, rows, codebook_rows, plan.part_len, items, plan.parts};
+    const size_t smem = kTileWarps * (kTilePieces * 32 * sizeof(uint4) +
+                                      (plan.lanes == 32 && top_k > 1 ? sizeof(TopSmem) : 0));
     with_tile_lanes(plan.lanes, [&](auto l) {
-      launch_pdl(k_log_probs<T, decltype(l)::value>, tile_blocks(items), kTileWarps * 32, 0, s, t, cd, top_k, o,
+      launch_pdl(k_log_probs<T, decltype(l)::value>, plan.blocks(rows), kTileWarps * 32, smem, s, t, cd, top_k, o,
                  b.stat, b.keys, status);
     });
     if (plan.parts > 1) {

@@ -155,12 +155,22 @@ __device__ __forceinline__ void load_row(const T* __restrict__ p, const Deal<T, 
 template <typename T, Mode M>
 __device__ __forceinline__ void load_row_single(const T* __restrict__ p, const Deal<T, M>& at,
                                                 float (&z)[kRowElems]) {
+  constexpr int VEC = Deal<T, M>::VEC;
   T q[kRowElems];
 #pragma unroll
-  for (int k = 0; k < kRowElems; ++k) {
-    const int c = at.index(k);
-    q[k] = from_f32<T>(0.0f);
-    if (at.has(c)) q[k] = p[c];
+  for (int v = 0; v < kRowElems / VEC; ++v) {
+    const int c = at.index(v * VEC);
+    if (at.whole(c)) {
+      const T* pc = p + c;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) q[v * VEC + i] = pc[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        q[v * VEC + i] = from_f32<T>(0.0f);
+        if (at.has(c + i)) q[v * VEC + i] = p[c + i];
+      }
+    }
   }
 #pragma unroll
   for (int k = 0; k < kRowElems; ++k) z[k] = to_f32(q[k]);
@@ -212,11 +222,18 @@ struct Counts {
       n[0] = q.x, n[1] = q.y, n[2] = q.z, n[3] = q.w;
     } else if constexpr (M == Mode::kShifted) {
       static_assert(Deal<T, M>::VEC == 8, "values of two bytes");
+      // The same residue modulo 8 in every lane: c + i = 8 q + j - shift.
+      const int q = (c - k % 8 + at.shift) >> 3;
+      if (at.whole(c - k % 8)) {
+        const float* p = by_eight + q;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // The same residue modulo 8 in every lane.
-        n[i] = 0.0f;
-        if (at.has(c + i)) n[i] = by_eight[((k % 8 + i - at.shift) & 7) * eights + ((c + i) >> 3)];
+        for (int i = 0; i < 4; ++i) {
+          const int j = k % 8 + i;
+          n[i] = p[((j - at.shift) & 7) * eights - (j < at.shift ? 1 : 0)];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n[i] = at.has(c + i) ? by_code[c + i] : 0.0f;
       }
     } else {
 #pragma unroll
@@ -251,15 +268,40 @@ __device__ __forceinline__ RowStat join(RowStat x, RowStat y) {
   if (e > 0.0f) r.w = hi.w + e * fmaf(kCounts ? lo.n - hi.n : d, one, lo.w);
   return r;
 }
-template <bool kCounts>
-__device__ __forceinline__ RowStat shuffle_join(RowStat x, int offset, int width) {
-  RowStat y;
-  y.m = __shfl_xor_sync(kFullMask, x.m, offset, width);
-  y.s = __shfl_xor_sync(kFullMask, x.s, offset, width);
-  y.w = __shfl_xor_sync(kFullMask, x.w, offset, width);
-  y.n = kCounts ? __shfl_xor_sync(kFullMask, x.n, offset, width) : 0.0f;
-  y.a = __shfl_xor_sync(kFullMask, x.a, offset, width);
-  return join<kCounts>(x, y);
+// Of the parts that WIDTH lanes hold: the same rule, with the largest value found
+// first, so that every part moves once.
+template <bool kCounts, int WIDTH>
+__device__ __forceinline__ RowStat join_lanes(const RowStat& x) {
+  RowStat r;
+  r.m = x.m;
+#pragma unroll
+  for (int o = WIDTH / 2; o > 0; o >>= 1) r.m = fmaxf(r.m, __shfl_xor_sync(kFullMask, r.m, o, WIDTH));
+  r.a = x.m == r.m ? x.a : 0xffffffffu;
+  if (WIDTH == 32) {
+    r.a = __reduce_min_sync(kFullMask, r.a);
+  } else {
+#pragma unroll
+    for (int o = WIDTH / 2; o > 0; o >>= 1) r.a = min(r.a, __shfl_xor_sync(kFullMask, r.a, o, WIDTH));
+  }
+  const bool winner = x.m == r.m && x.a == r.a;
+  r.n = 0.0f;
+  if (kCounts) {
+    r.n = winner ? x.n : neg_inf();
+#pragma unroll
+    for (int o = WIDTH / 2; o > 0; o >>= 1) r.n = fmaxf(r.n, __shfl_xor_sync(kFullMask, r.n, o, WIDTH));
+  }
+  const float d = x.m - r.m;  // NaN where both are -inf: nothing to move then
+  const float e = x.m == neg_inf() ? 0.0f : ex2_approx(d * kLog2e);
+  const float one = 1.0f + x.s;
+  r.s = e == 0.0f ? 0.0f * x.s : e * one;  // 0 * NaN: a NaN stays
+  r.w = e > 0.0f ? e * fmaf(kCounts ? x.n - r.n : d, one, x.w) : 0.0f;
+  if (winner) r.s = x.s, r.w = x.w;
+#pragma unroll
+  for (int o = WIDTH / 2; o > 0; o >>= 1) {
+    r.s += __shfl_xor_sync(kFullMask, r.s, o, WIDTH);
+    r.w += __shfl_xor_sync(kFullMask, r.w, o, WIDTH);
+  }
+  return r;
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {  // NaN loses against any number

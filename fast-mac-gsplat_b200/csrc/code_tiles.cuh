@@ -2,37 +2,34 @@
 // rows that stream through shared memory.
 //
 // A warp owns its rows from the first load to the result: no block-wide barrier.
-//   - L = 2 .. 16 lanes a row, 32 / L rows at once, for rows that fit 8 pieces of
-//     16 bytes a lane;
-//   - L = 32 for longer rows (or parts of a row), which pass in slices of 8 pieces a
+//   - L = 1 .. 16 lanes a row, 32 / L rows at once, for rows that fit 16 pieces of 16
+//     bytes a lane (what a row costs besides its values is paid once for all of them);
+//   - L = 32 for longer rows (or parts of a row), which pass in slices of 16 pieces a
 //     lane; every lane keeps its own maximum and sums over the slices, so that lanes
 //     exchange values once a row.
-// Slices are copied asynchronously, one ahead of the one in work, and each lane reads only what it copied itself, which needs no barrier either. Shared
-// memory also gives a lane's values an index: the largest one is found by piece and
-// taken out of the sums by one store, where values in registers cost a comparison
-// and a selection each.
+// Pieces are copied asynchronously and each lane reads only what it copied itself,
+// which needs no barrier either. A warp's buffer is refilled from the next slice four
+// pieces at a time as the sums pass over it. Shared memory also gives a lane's values
+// an index: the largest one is found by piece and taken out of the sums by one store,
+// where values in registers cost a comparison and a selection each.
 //
 // Bound by the logits' bytes while a value costs no more than a few instructions: a
-// maximum (two values at a time for 16-bit types), a conversion, and half of each of
-// an FMA, an addition and an FMA on pairs around one ex2.
+// maximum and a minimum (of two values at a time for 16-bit types), a conversion, and
+// half of each of an FMA, an addition and an FMA on pairs around one ex2.
 #pragma once
 
 #include "code_rows.cuh"
 
 namespace gsb {
 
-constexpr int kTilePieces = 8;  // of 16 bytes, a lane
-constexpr int kTileStages = 2;  // one in work, one on its way
-constexpr int kTileWarps = 4;   // a block
-constexpr int kTileSlices = 8;  // a part, at most
-
-template <typename T>
-constexpr int tile_elems() { return kTilePieces * wide_of<T>(); }  // values a lane
+constexpr int kTileWarps = 4;    // a block
+constexpr int kTilePieces = 16;  // of a lane
+constexpr int kTileGroup = 4;    // pieces that are worked on and refilled together
 
 // Where a lane's values of a slice lie: piece v's value i has the index at(v) + i in
 // its part (or row) of len values. shift: values between the 16-byte boundary before
 // the part and its start. Pieces w0 .. w1 - 1 are whole for every lane of the row; of
-// the n that any lane has, those beside them are ragged: at most the first and the last.
+// the n (a multiple of kTileGroup) in work, the others are ragged or empty.
 template <typename T, int L>
 struct Slice {
   static constexpr int VEC = wide_of<T>();
@@ -44,15 +41,17 @@ struct Slice {
     first = begin + lane * VEC;
     w0 = begin < 0 ? 1 : 0;
     w1 = min(left / (L * VEC), kTilePieces);
-    n = min((left + L * VEC - 1) / (L * VEC), kTilePieces);
+    constexpr int kGroupValues = L * VEC * kTileGroup;
+    n = min((left + kGroupValues - 1) / kGroupValues * kTileGroup, kTilePieces);
+    if (L < 32) n = __reduce_max_sync(kFullMask, n);  // rows may lie differently; a warp goes through as many pieces
   }
   __device__ __forceinline__ int at(int v) const { return first + v * L * VEC; }
   __device__ __forceinline__ bool has(int c) const { return c >= 0 && c < len; }
   __device__ __forceinline__ bool ragged() const { return w0 > 0 || w1 < n; }
-  // Calls fn(v) for the ragged pieces.
+  // Calls fn(v) for the pieces that are not whole.
   template <typename Fn>
   __device__ __forceinline__ void each_ragged(Fn&& fn) const {
-    for (int v = w0 > 0 ? 0 : w1; v < n; v = v < w1 ? w1 : n) fn(v);
+    for (int v = w0 > 0 ? 0 : w1; v < n; v = v + 1 < w1 && v < w1 ? w1 : v + 1) fn(v);
   }
 };
 
@@ -61,38 +60,60 @@ __device__ __forceinline__ void cp_async16_part(void* smem, const void* gmem, in
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(s), "l"(gmem), "r"(bytes) : "memory");
 }
 
-// Begins the copy of a lane's pieces of a slice. A piece may reach in front of its
-// row, into the row before (its values are not used), but not in front of `base`,
-// the logits' first value: the few values of such a piece are copied one by one.
+// A lane's pieces in its warp's buffer; piece v of the lanes lie side by side.
+struct LaneBuf {
+  uint4* base;
+  __device__ __forceinline__ uint4& operator[](int v) const { return base[v * 32]; }
+};
+
+// Begins the copy of the whole pieces v0 .. v0 + kTileGroup - 1 of a lane.
 template <typename T, int L>
-__device__ __forceinline__ void issue_slice(uint4* buf, const T* __restrict__ p, const T* __restrict__ base,
+__device__ __forceinline__ void copy_group(const LaneBuf& buf, const T* __restrict__ p, const Slice<T, L>& at, int v0) {
+  constexpr int VEC = wide_of<T>();
+  const T* from = p + at.first + v0 * L * VEC;
+  if (v0 >= at.w0 && v0 + kTileGroup <= at.w1) {
+#pragma unroll
+    for (int v = 0; v < kTileGroup; ++v) cp_async16(&buf[v0 + v], from + v * L * VEC);
+  } else {
+    for (int v = v0; v < v0 + kTileGroup; ++v)
+      if (v >= at.w0 && v < at.w1) cp_async16(&buf[v], p + at.at(v));
+  }
+}
+// Begins the copy of the ragged pieces. A piece may reach in front of its row, into
+// the row before (its values are not used), but not in front of `base`, the logits'
+// first value: the few values of such a piece are copied one by one.
+template <typename T, int L>
+__device__ __forceinline__ void copy_ragged(const LaneBuf& buf, const T* __restrict__ p, const T* __restrict__ base,
                                             const Slice<T, L>& at) {
   constexpr int VEC = wide_of<T>();
-  const T* from = p + at.first;
-#pragma unroll
-  for (int v = 0; v < kTilePieces; ++v)
-    if (v >= at.w0 && v < at.w1) cp_async16(buf + v * 32, from + v * L * VEC);
-  if (at.ragged()) {
-    at.each_ragged([&](int v) {
-      const int c = at.at(v);
-      uint4* to = buf + v * 32;
-      if (c >= at.len || c + VEC <= 0) return;
-      if (c < 0 && p + c < base) {
-        for (int i = 0; i < VEC; ++i)
-          if (at.has(c + i)) reinterpret_cast<T*>(to)[i] = p[c + i];
-      } else {
-        cp_async16_part(to, p + c, min(VEC, at.len - c) * (int)sizeof(T));
-      }
-    });
-  }
+  if (!at.ragged()) return;
+  at.each_ragged([&](int v) {
+    const int c = at.at(v);
+    uint4* to = &buf[v];
+    if (c >= at.len || c + VEC <= 0) return;
+    if (c < 0 && p + c < base) {
+      for (int i = 0; i < VEC; ++i)
+        if (at.has(c + i)) reinterpret_cast<T*>(to)[i] = p[c + i];
+    } else {
+      cp_async16_part(to, p + c, min(VEC, at.len - c) * (int)sizeof(T));
+    }
+  });
 }
 // Puts `value` in the places of ragged pieces that hold none of the part's values.
 template <typename T, int L>
-__device__ __forceinline__ void fill_ragged(uint4* buf, const Slice<T, L>& at, float value) {
-  const T e = from_f32<T>(value);
+__device__ __forceinline__ void fill_ragged(const LaneBuf& buf, const Slice<T, L>& at, float value) {
+  constexpr int VEC = wide_of<T>();
+  T e[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) e[i] = from_f32<T>(value);
   at.each_ragged([&](int v) {
-    for (int i = 0; i < wide_of<T>(); ++i)
-      if (!at.has(at.at(v) + i)) reinterpret_cast<T*>(buf + v * 32)[i] = e;
+    const int c = at.at(v);
+    if (c >= at.len || c + VEC <= 0) {
+      buf[v] = *reinterpret_cast<const uint4*>(e);
+    } else if (c < 0 || c + VEC > at.len) {
+      for (int i = 0; i < VEC; ++i)
+        if (!at.has(c + i)) reinterpret_cast<T*>(&buf[v])[i] = e[0];
+    }
   });
 }
 
@@ -102,67 +123,99 @@ __device__ __forceinline__ void unpack(const uint4& q, float (&f)[wide_of<T>()])
 #pragma unroll
   for (int i = 0; i < wide_of<T>(); ++i) f[i] = to_f32(e[i]);
 }
-// Largest and smallest value of a piece (NaN loses against any).
-__device__ __forceinline__ void piece_range(const uint4& q, float, float& hi, float& lo) {
-  const float a = __uint_as_float(q.x), b = __uint_as_float(q.y), c = __uint_as_float(q.z), d = __uint_as_float(q.w);
-  hi = fmaxf(max3(a, b, c), d);
-  lo = fminf(min3(a, b, c), d);
-}
-__device__ __forceinline__ void piece_range(const uint4& q, __nv_bfloat16, float& hi, float& lo) {
-  const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&q);
-  const __nv_bfloat162 h = __hmax2(__hmax2(e[0], e[1]), __hmax2(e[2], e[3]));
-  const __nv_bfloat162 l = __hmin2(__hmin2(e[0], e[1]), __hmin2(e[2], e[3]));
-  hi = fmaxf(__low2float(h), __high2float(h));
-  lo = fminf(__low2float(l), __high2float(l));
-}
-__device__ __forceinline__ void piece_range(const uint4& q, __half, float& hi, float& lo) {
-  const __half2* e = reinterpret_cast<const __half2*>(&q);
-  const __half2 h = __hmax2(__hmax2(e[0], e[1]), __hmax2(e[2], e[3]));
-  const __half2 l = __hmin2(__hmin2(e[0], e[1]), __hmin2(e[2], e[3]));
-  hi = fmaxf(__low2float(h), __high2float(h));
-  lo = fminf(__low2float(l), __high2float(l));
-}
 
-// Counts of a piece's values; 0 where the part has none.
+// Largest and smallest value (NaN loses against any) of pieces, 16-bit types two at a
+// time.
+template <typename T>
+struct Range;
+template <>
+struct Range<float> {
+  float hi, lo;
+  __device__ __forceinline__ explicit Range(const uint4& q) {
+    const float a = __uint_as_float(q.x), b = __uint_as_float(q.y), c = __uint_as_float(q.z),
+                d = __uint_as_float(q.w);
+    hi = fmaxf(max3(a, b, c), d);
+    lo = fminf(min3(a, b, c), d);
+  }
+  __device__ __forceinline__ void add(const Range& r) { hi = fmaxf(hi, r.hi), lo = fminf(lo, r.lo); }
+  __device__ __forceinline__ float top() const { return hi; }
+  __device__ __forceinline__ float low() const { return lo; }
+};
+template <typename P>
+struct PairRange {
+  P hi, lo;
+  __device__ __forceinline__ explicit PairRange(const uint4& q) {
+    const P* e = reinterpret_cast<const P*>(&q);
+    hi = __hmax2(__hmax2(e[0], e[1]), __hmax2(e[2], e[3]));
+    lo = __hmin2(__hmin2(e[0], e[1]), __hmin2(e[2], e[3]));
+  }
+  __device__ __forceinline__ void add(const PairRange& r) { hi = __hmax2(hi, r.hi), lo = __hmin2(lo, r.lo); }
+  __device__ __forceinline__ float top() const { return fmaxf(__low2float(hi), __high2float(hi)); }
+  __device__ __forceinline__ float low() const { return fminf(__low2float(lo), __high2float(lo)); }
+};
+template <>
+struct Range<__nv_bfloat16> : PairRange<__nv_bfloat162> {
+  using PairRange::PairRange;
+};
+template <>
+struct Range<__half> : PairRange<__half2> {
+  using PairRange::PairRange;
+};
+
+// Counts of the values of the pieces v0 .. v0 + kTileGroup - 1; 0 where the part has none.
 template <typename T, int L>
-__device__ __forceinline__ void piece_counts(const Counts& counts, const Slice<T, L>& at, int v,
-                                             float (&n)[wide_of<T>()]) {
+__device__ __forceinline__ void group_counts(const Counts& counts, const Slice<T, L>& at, int v0,
+                                             float (&n)[kTileGroup][wide_of<T>()]) {
   constexpr int VEC = wide_of<T>();
-  const int c = at.at(v);
-  if (at.shift == 0) {
+  if (at.shift == 0 && v0 + kTileGroup <= at.w1) {
+    const float4* p = reinterpret_cast<const float4*>(counts.by_code + at.at(v0));
 #pragma unroll
-    for (int i = 0; i < VEC; i += 4) {
-      // Padded to a multiple of 8 codes: a piece that the part has any of is all there.
-      const float4 q = c < at.len ? *reinterpret_cast<const float4*>(counts.by_code + c + i)
-                                  : make_float4(0.f, 0.f, 0.f, 0.f);
-      n[i] = q.x, n[i + 1] = q.y, n[i + 2] = q.z, n[i + 3] = q.w;
-    }
-  } else {
+    for (int v = 0; v < kTileGroup; ++v)
+#pragma unroll
+      for (int i = 0; i < VEC; i += 4) {
+        const float4 q = p[(v * L * VEC + i) / 4];
+        n[v][i] = q.x, n[v][i + 1] = q.y, n[v][i + 2] = q.z, n[v][i + 3] = q.w;
+      }
+  } else if (VEC == 8 && v0 >= at.w0 && v0 + kTileGroup <= at.w1) {
+    // Codes of one residue modulo 8 lie side by side, as the lanes' pieces of 8 do.
+    const float* p = counts.by_eight + ((at.at(v0) + at.shift) >> 3);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      n[i] = 0.0f;
-      if (at.has(c + i))
-        n[i] = VEC == 8 ? counts.by_eight[((i - at.shift) & 7) * counts.eights + ((c + i) >> 3)]
-                        : counts.by_code[c + i];
+      const float* pi = p + (((i - at.shift) & 7) * counts.eights - (i < at.shift ? 1 : 0));
+#pragma unroll
+      for (int v = 0; v < kTileGroup; ++v) n[v][i] = pi[v * L];
+    }
+  } else {
+    for (int v = 0; v < kTileGroup; ++v) {
+      const int c = at.at(v0 + v);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float q = at.has(c + i) ? counts.by_code[c + i] : 0.0f;
+#pragma unroll
+        for (int u = 0; u < kTileGroup; ++u)
+          if (u == v) n[u][i] = q;
+      }
     }
   }
 }
 
 // The sums of a lane's pieces about base.m (r.n: the count that others are taken
 // relative to). kClamp: some value is -inf, or so low that its multiple with log2 e
-// is; e = 0 times that would be NaN.
-template <bool kCounts, bool kClamp, typename T, int L>
-__device__ __forceinline__ void piece_sums(const uint4* buf, const Slice<T, L>& at, const Counts& counts,
-                                           const Base& base, RowStat& r) {
+// is; e = 0 times that would be NaN. done(v) is called when pieces v .. v +
+// kTileGroup - 1 are not needed any more.
+template <bool kCounts, bool kClamp, typename T, int L, typename Done>
+__device__ __forceinline__ void piece_sums(const LaneBuf& buf, const Slice<T, L>& at, const Counts& counts,
+                                           const Base& base, RowStat& r, Done&& done) {
   constexpr int VEC = wide_of<T>();
   const F2 l2 = f2(kLog2e), neg_M = f2(base.neg_M), neg_n = f2(-r.n);
   F2 s2 = f2(0.0f), w2 = f2(0.0f);
+  for (int v0 = 0; v0 < at.n; v0 += kTileGroup) {
+    float n[kTileGroup][VEC];
+    if constexpr (kCounts) group_counts(counts, at, v0, n);
 #pragma unroll
-  for (int v = 0; v < kTilePieces; ++v) {
-    if (v < at.n) {
-      float f[VEC], n[VEC];
-      if constexpr (kCounts) piece_counts(counts, at, v, n);
-      unpack<T>(buf[v * 32], f);
+    for (int v = 0; v < kTileGroup; ++v) {
+      float f[VEC];
+      unpack<T>(buf[v0 + v], f);
 #pragma unroll
       for (int i = 0; i < VEC; i += 2) {
         F2 y = fma2(f2(f[i], f[i + 1]), l2, neg_M);
@@ -174,9 +227,10 @@ __device__ __forceinline__ void piece_sums(const uint4* buf, const Slice<T, L>& 
         }
         const F2 e = f2(ex2_approx(y0), ex2_approx(y1));
         s2 = add2(s2, e);
-        w2 = fma2(e, kCounts ? add2(f2(n[i], n[i + 1]), neg_n) : y, w2);
+        w2 = fma2(e, kCounts ? add2(f2(n[v][i], n[v][i + 1]), neg_n) : y, w2);
       }
     }
+    done(v0);
   }
   float s0, s1, w0, w1;
   split(s2, s0, s1);
@@ -188,66 +242,105 @@ __device__ __forceinline__ void piece_sums(const uint4* buf, const Slice<T, L>& 
   r.s *= base.undo;
 }
 
-// The softmax sums of one lane's values of a slice (buf: its pieces, 32 apart),
-// without its largest (its first largest, which leaves `buf` too). The index in the
-// result is the part's.
-template <bool kCounts, typename T, int L>
-__device__ __forceinline__ RowStat lane_sums(uint4* buf, const Slice<T, L>& at, const Counts& counts) {
+// The largest of a lane's pieces: its value (NaN: there is none) and group, the
+// largest of the other groups, and the smallest. group_top(v, top) is told each
+// group's largest.
+struct LaneTop {
+  float m, rest, low;
+  int group;
+};
+template <typename T, int L, typename GroupTop>
+__device__ __forceinline__ LaneTop lane_top(const LaneBuf& buf, const Slice<T, L>& at, GroupTop&& group_top) {
+  LaneTop t{quiet_nan(), quiet_nan(), 0.0f, 0};
+  for (int v0 = 0; v0 < at.n; v0 += kTileGroup) {
+    Range<T> range(buf[v0]);
+#pragma unroll
+    for (int v = 1; v < kTileGroup; ++v) range.add(Range<T>(buf[v0 + v]));
+    const float top = range.top();
+    t.low = fminf(t.low, range.low());
+    const bool first = top > t.m || t.m != t.m;  // the first of equal ones
+    t.rest = fmaxf(t.rest, first ? t.m : top);
+    if (first) t.m = top, t.group = v0;
+    group_top(v0, top);
+  }
+  return t;
+}
+// The first place of the value m in a group of a lane's pieces, and the largest of
+// the group's other values.
+template <typename T>
+__device__ __forceinline__ void find_value(const LaneBuf& buf, int v0, float m, int* v_out, int* i_out, float* rest) {
+  constexpr int VEC = wide_of<T>();
+  float top[kTileGroup];
+#pragma unroll
+  for (int v = 0; v < kTileGroup; ++v) top[v] = Range<T>(buf[v0 + v]).top();
+  int v_at = kTileGroup - 1;
+#pragma unroll
+  for (int v = kTileGroup - 2; v >= 0; --v)
+    if (top[v] == m) v_at = v;
+  float f[VEC], other = quiet_nan();
+#pragma unroll
+  for (int v = 0; v < kTileGroup; ++v) other = fmaxf(other, v == v_at ? quiet_nan() : top[v]);
+  unpack<T>(buf[v0 + v_at], f);
+  int i_at = 0;
+#pragma unroll
+  for (int i = VEC - 1; i >= 0; --i)
+    if (f[i] == m) i_at = i;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) other = fmaxf(other, i == i_at ? quiet_nan() : f[i]);
+  *v_out = v0 + v_at;
+  *i_out = i_at;
+  *rest = other;
+}
+
+// The softmax sums of one lane's values of a slice, without its largest (its first largest, which leaves `buf` too). The index in the
+// result is the part's. second: the largest of the others (NaN: none).
+template <bool kCounts, typename T, int L, typename GroupTop, typename Done>
+__device__ __forceinline__ RowStat lane_sums(const LaneBuf& buf, const Slice<T, L>& at, const Counts& counts, float& second,
+                                             GroupTop&& group_top, Done&& done) {
   constexpr int VEC = wide_of<T>();
   if (at.ragged()) fill_ragged(buf, at, quiet_nan());
-  float top[kTilePieces], low = 0.0f;
-#pragma unroll
-  for (int v = 0; v < kTilePieces; ++v) {
-    top[v] = quiet_nan();
-    if (v < at.n) {
-      float lo;
-      piece_range(buf[v * 32], T{}, top[v], lo);
-      low = fminf(low, lo);
-    }
-  }
+  const LaneTop top = lane_top(buf, at, group_top);
   RowStat r;
-  const float m = max3(max3(top[0], top[1], top[2]), max3(top[3], top[4], top[5]), fmaxf(top[6], top[7]));
-  const bool some = m == m;                   // else: no value, or NaN alone
-  const Base base(m > neg_inf() ? m : 0.0f);  // with m = -inf all is 0 (or NaN) relative to 0 too
+  const bool some = top.m == top.m;                   // else: no value, or NaN alone
+  const Base base(top.m > neg_inf() ? top.m : 0.0f);  // with m = -inf all is 0 (or NaN) relative to 0 too
   const float none = base.far ? neg_inf() : base.m - 200.0f;  // adds nothing
   r.a = 0xffffffffu;
+  second = quiet_nan();
   if (some) {
-    int v0 = 0;
-#pragma unroll
-    for (int v = kTilePieces - 1; v >= 0; --v)
-      if (top[v] == m) v0 = v;
-    float f[VEC];
-    unpack<T>(buf[v0 * 32], f);
-    int i0 = 0;
-#pragma unroll
-    for (int i = VEC - 1; i >= 0; --i)
-      if (f[i] == m) i0 = i;
-    reinterpret_cast<T*>(buf + v0 * 32)[i0] = from_f32<T>(none);
-    r.a = (uint32_t)(at.at(v0) + i0);
+    int v, i;
+    find_value<T>(buf, top.group, top.m, &v, &i, &second);
+    second = fmaxf(second, top.rest);
+    reinterpret_cast<T*>(&buf[v])[i] = from_f32<T>(none);
+    r.a = (uint32_t)(at.at(v) + i);
   }
   if (at.ragged()) fill_ragged(buf, at, none);
   r.n = kCounts && some ? counts.by_code[r.a] : 0.0f;
   if (__any_sync(kFullMask, base.far)) {
     r.s = r.w = 0.0f;
-    for (int v = 0; v < at.n; ++v) {
-      float f[VEC], n[VEC];
-      unpack<T>(buf[v * 32], f);
-      if constexpr (kCounts) piece_counts(counts, at, v, n);
+    for (int v0 = 0; v0 < at.n; v0 += kTileGroup) {
+      float n[kTileGroup][VEC];
+      if constexpr (kCounts) group_counts(counts, at, v0, n);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float x = max_nan(f[i] - base.m, -200.0f);
-        const float e = ex2_approx(x * kLog2e);
-        r.s += e;
-        r.w = fmaf(e, kCounts ? n[i] - r.n : x, r.w);
+      for (int v = 0; v < kTileGroup; ++v) {
+        float f[VEC];
+        unpack<T>(buf[v0 + v], f);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float x = max_nan(f[i] - base.m, -200.0f);
+          const float e = ex2_approx(x * kLog2e);
+          r.s += e;
+          r.w = fmaf(e, kCounts ? n[v][i] - r.n : x, r.w);
+        }
       }
+      done(v0);
     }
-  } else if (!kCounts && __any_sync(kFullMask, low < kLowest)) {
-    piece_sums<kCounts, !kCounts>(buf, at, counts, base, r);
+  } else if (!kCounts && __any_sync(kFullMask, top.low < kLowest)) {
+    piece_sums<kCounts, !kCounts>(buf, at, counts, base, r, done);
   } else {
-    piece_sums<kCounts, false>(buf, at, counts, base, r);
+    piece_sums<kCounts, false>(buf, at, counts, base, r, done);
   }
-  const bool lane_any = at.first < at.len && at.first + (kTilePieces - 1) * L * VEC + VEC > 0;
-  r.m = some ? m : neg_inf();
+  const bool lane_any = at.first < at.len && at.at(at.n - 1) + VEC > 0;
+  r.m = some ? top.m : neg_inf();
   if (!some) {
     r.w = 0.0f;
     if (!lane_any) r.s = 0.0f;
@@ -259,48 +352,58 @@ __device__ __forceinline__ RowStat lane_sums(uint4* buf, const Slice<T, L>& at, 
 struct TilePlan {
   int lanes = 32;
   int parts = 1;
+  int blocks_sm = 1;
   int64_t part_len = 0;
+  int blocks(int64_t rows) const {
+    return (int)std::min<int64_t>(148 * blocks_sm, (items(rows) + kTileWarps - 1) / kTileWarps);
+  }
   int64_t items(int64_t rows) const { return lanes < 32 ? (rows + 32 / lanes - 1) / (32 / lanes) : rows * parts; }
 };
-// Rows that fit 16 lanes share a warp. Longer ones take a warp a part; parts of
-// kTileSlices slices at most, or shorter ones where there are too few rows for two
-// rounds of the warps that are resident, but none below a slice.
-// shifted: rows may begin between 16-byte boundaries.
-inline TilePlan tile_plan(int64_t rows, int64_t codes, int size, bool shifted) {
+// Rows that fit 16 lanes share a warp (shifted: they may begin between 16-byte
+// boundaries). Longer ones take a warp a part; there are as many parts as make the
+// longest warp's way shortest, a part costing a quarter of a slice besides its
+// values. most_slices: of a part; blocks_sm: blocks that an SM holds (of the kernels
+// for short rows: blocks_sm_short).
+inline TilePlan tile_plan(int64_t rows, int64_t codes, int size, bool shifted, int64_t most_slices, int blocks_sm,
+                          int blocks_sm_short) {
   TilePlan p;
-  const int vec = 16 / size, elems = kTilePieces * vec;
+  p.blocks_sm = blocks_sm;
+  const int64_t resident = 148 * blocks_sm * kTileWarps;
+  const int vec = 16 / size;
   p.part_len = codes;
-  for (int l = 2; l <= 16; l *= 2) {
-    if (codes + (shifted ? vec - 1 : 0) <= l * elems) {
+  for (int l = 1; l <= 16; l *= 2) {
+    if (codes + (shifted ? vec - 1 : 0) <= l * kTilePieces * vec) {
       p.lanes = l;
+      p.blocks_sm = blocks_sm_short;
       return p;
     }
   }
-  const int64_t slice = 32 * elems, most = kTileSlices * slice - 8;
-  int64_t parts = (codes + most - 1) / most;
-  constexpr int64_t kFill = 2 * 148 * 16;
-  if (rows * parts < kFill) parts = std::max(parts, std::min((codes + slice - 1) / slice, (kFill + rows - 1) / rows));
-  p.part_len = ((codes + parts - 1) / parts + 7) / 8 * 8;
+  const int64_t slice = 32 * kTilePieces * vec, most = most_slices * slice - 8;
+  const int64_t least_parts = (codes + most - 1) / most;
+  const int64_t most_parts = std::max(least_parts, std::min<int64_t>((codes + slice / 4 - 1) / (slice / 4), 1024));
+  int64_t best_cost = INT64_MAX, best = least_parts;
+  for (int64_t parts = least_parts; parts <= most_parts; ++parts) {
+    const int64_t rounds = (rows * parts + resident - 1) / resident;
+    const int64_t cost = rounds * ((codes + parts - 1) / parts + slice / 4) + (parts > 1 ? slice / 2 : 0);
+    if (cost < best_cost) best_cost = cost, best = parts;
+    if (rounds > 8) break;  // even enough from here on
+  }
+  p.part_len = ((codes + best - 1) / best + 7) / 8 * 8;
   p.parts = (int)((codes + p.part_len - 1) / p.part_len);
   return p;
 }
 template <typename Fn>
 inline void with_tile_lanes(int lanes, Fn&& fn) {
-  if (lanes == 2) fn(std::integral_constant<int, 2>{});
+  if (lanes == 1) fn(std::integral_constant<int, 1>{});
+  else if (lanes == 2) fn(std::integral_constant<int, 2>{});
   else if (lanes == 4) fn(std::integral_constant<int, 4>{});
   else if (lanes == 8) fn(std::integral_constant<int, 8>{});
   else if (lanes == 16) fn(std::integral_constant<int, 16>{});
   else fn(std::integral_constant<int, 32>{});
 }
-
 inline bool rows_shifted(int size, const void* p, int64_t stride) {
   return reinterpret_cast<uintptr_t>(p) % 16 != 0 || stride * size % 16 != 0;
 }
-inline int tile_blocks(int64_t items) {
-  constexpr int kResident = 148 * 5;  // by shared memory
-  return (int)std::min<int64_t>(kResident, (items + kTileWarps - 1) / kTileWarps);
-}
-
 // The rows of a call, and where a warp is in them.
 template <typename T>
 struct TileRows {
@@ -312,9 +415,9 @@ template <typename T, int L>
 struct TilePlace {
   int64_t item, row, c0;
   const T* p;  // the part's first value
-  int slice, slices, len, shift;
+  int slices, len, shift;
   bool on;
-  __device__ __forceinline__ TilePlace(const TileRows<T>& t, int64_t item_, int lane32) : item(item_), slice(0) {
+  __device__ __forceinline__ TilePlace(const TileRows<T>& t, int64_t item_, int lane32) : item(item_) {
     if (L < 32) {
       const int64_t mine = item * (32 / L) + lane32 / L;
       on = mine < t.rows;
@@ -329,47 +432,66 @@ struct TilePlace {
     }
     p = t.logits + row * t.stride + c0;
     shift = (int)(reinterpret_cast<uintptr_t>(p) % 16 / sizeof(T));
-    constexpr int kSlice = L * tile_elems<T>();
+    constexpr int kSlice = L * kTilePieces * wide_of<T>();
     slices = L < 32 ? 1 : (len + shift + kSlice - 1) / kSlice;
   }
-  __device__ __forceinline__ Slice<T, L> values(int lane32) const { return Slice<T, L>(len, shift, slice, lane32 % L); }
+  __device__ __forceinline__ Slice<T, L> values(int slice, int lane32) const {
+    return Slice<T, L>(len, shift, slice, lane32 % L);
+  }
 };
 
-// Takes a warp through its items, slice by slice: work(place, buffer) once a slice is
-// there (buffer: the lane's pieces); ahead(place) a slice's work before an item's first one (for loads that the
-// item will want), turn() between the last slice of an item and the next item.
-template <typename T, int L, typename Ahead, typename Turn, typename Work>
-__device__ __forceinline__ void walk_tiles(const TileRows<T>& t, uint4* warp_buf, int lane32, Ahead&& ahead, Turn&& turn,
-                                           Work&& work) {
-  constexpr int kStage = kTilePieces * 32;
-  uint4* buf = warp_buf + lane32;  // a lane's pieces lie 32 apart
+// Takes a warp through its items. For each: ahead(place), once, before the item's
+// first copy is waited for (for loads that it will want); then for each slice
+// work(place, slice, values, buffer, refill), whose refill is the `done` of lane_sums;
+// last turn(place, values, buffer). hold: turn wants the last slice's values still; the
+// next item's copy begins after it.
+template <typename T, int L, typename Ahead, typename Work, typename Turn>
+__device__ __forceinline__ void walk_tiles(const TileRows<T>& t, uint4* warp_buf, int lane32, bool hold, Ahead&& ahead,
+                                           Work&& work, Turn&& turn) {
+  const LaneBuf buf{warp_buf + lane32};
   const int64_t step = (int64_t)gridDim.x * kTileWarps;
-  const int64_t first = (int64_t)blockIdx.x * kTileWarps + threadIdx.x / 32;
-  if (first >= t.items) return;
-  TilePlace<T, L> now(t, first, lane32);
-  ahead(now);
-  turn();
-  issue_slice<T, L>(buf, now.p, t.logits, now.values(lane32));
-  cp_async_commit();
-  int stage = 0;
-  for (bool more = true; more;) {
-    TilePlace<T, L> next = now;
-    if (++next.slice == now.slices) {
-      more = now.item + step < t.items;
-      if (more) next = TilePlace<T, L>(t, now.item + step, lane32);
-    }
-    // The lane's accesses to the buffer that the copy goes to come before it.
-    __syncwarp();
-    if (more) issue_slice<T, L>(buf + (stage ^ 1) * kStage, next.p, t.logits, next.values(lane32));
+  int64_t item = (int64_t)blockIdx.x * kTileWarps + threadIdx.x / 32;
+  if (item >= t.items) return;
+  TilePlace<T, L> now(t, item, lane32);
+  Slice<T, L> at = now.values(0, lane32);
+  // Groups from v0 on, and what is not whole.
+  auto copy_rest = [&](const TilePlace<T, L>& place, const Slice<T, L>& values, int v0) {
+    for (; v0 < values.n; v0 += kTileGroup) copy_group(buf, place.p, values, v0);
+    copy_ragged(buf, place.p, t.logits, values);
     cp_async_commit();
-    const bool new_item = more && next.slice == 0;
-    if (new_item) ahead(next);
-    cp_async_wait<1>();
+  };
+  ahead(now);
+  copy_rest(now, at, 0);
+  int slice = 0;
+  for (bool more = true; more;) {
+    cp_async_wait<0>();
     __syncwarp();
-    work(now, buf + stage * kStage);
-    if (new_item) turn();
+    const bool last = L < 32 || slice + 1 == now.slices;
+    TilePlace<T, L> next = now;
+    int next_slice = slice + 1;
+    if (last) {
+      item += step;
+      more = item < t.items;
+      next_slice = 0;
+      if (more) next = TilePlace<T, L>(t, item, lane32);
+    }
+    const Slice<T, L> next_at = next.values(next_slice, lane32);
+    const bool refill = more && !(hold && last);
+    work(now, slice, at, buf, [&](int v0) {
+      __syncwarp();  // what was read comes before the copy that replaces it
+      if (refill) copy_group(buf, next.p, next_at, v0);
+    });
+    __syncwarp();
+    if (refill) copy_rest(next, next_at, at.n);
+    if (last) {
+      turn(now, at, buf);
+      __syncwarp();
+      if (more && hold) copy_rest(next, next_at, 0);
+      if (more) ahead(next);
+    }
     now = next;
-    stage ^= 1;
+    at = next_at;
+    slice = next_slice;
   }
 }
 
