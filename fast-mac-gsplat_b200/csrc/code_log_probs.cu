@@ -345,91 +345,131 @@ struct LogProbsIn {
 };
 
 // dz_c = p_c (-lead - gH (z_c - m - mu)) + sum_i g_i [c = c_i], lead = sum_i g_i over the
-// given code and the alternatives. At the c_i, which are written a second time, the sum
-// is (sum of their g_i) (1 - p_c) - (sum of the other g_i) p_c.
-// `at` deals out the result's values of a stretch at c0 (SAME: the logits' lie alike);
-// sync() orders the two writes.
-template <bool SAME, typename T, Mode M, typename Sync>
-__device__ __forceinline__ void log_probs_grad(int64_t row, int64_t C, int c0, const Deal<T, M>& at, bool on,
-                                               const T* __restrict__ p, T* __restrict__ dz, const LogProbsIn& in,
-                                               Sync&& sync) {
-  const int len = at.len, lanes = at.lanes, lane = at.lane;
-  float z[kRowElems];
-  if constexpr (SAME) load_row(p + c0, at, 0u, z);
-  else load_row_single(p + c0, at, z);
-  const float4 st = in.stats[row];
-  const bool empty = st.x == neg_inf() && st.y == st.y;
-  const float inv = 1.0f / (1.0f + st.y);
-  int64_t code = in.g_log_probs ? in.codes.at(row) : -1;
-  if (code >= C) code = -1;
-  const float gl = code >= 0 ? in.g_log_probs[row] : 0.0f;
-  const float gh = in.g_entropy ? in.g_entropy[row] : 0.0f;
-  const int k = in.top_k;
-  const int32_t* tc = in.top_codes + row * k;
-  const float* gt = in.g_top + row * k;
-  float lead = gl;
-  for (int j = 0; j < k; ++j) lead += gt[j];
+// given code and the alternatives. The places c_i are written a second time, with
+// (sum of their g_i) (1 - p_c) - (sum of the other g_i) p_c for the sum.
+// Bound by the logits' and the gradient's bytes.
+struct RowGrad {
+  float4 st;
+  float inv, gl, gh, lead;
+  int64_t code;
+  bool empty;
+  __device__ __forceinline__ RowGrad(const LogProbsIn& in, int64_t row, int64_t C) {
+    st = in.stats[row];
+    code = in.g_log_probs ? in.codes.at(row) : -1;
+    if (code >= C) code = -1;
+    gl = code >= 0 ? in.g_log_probs[row] : 0.0f;
+    gh = in.g_entropy ? in.g_entropy[row] : 0.0f;
+    lead = gl;
+    for (int j = 0; j < in.top_k; ++j) lead += in.g_top[row * in.top_k + j];
+    empty = st.x == neg_inf() && st.y == st.y;
+    inv = 1.0f / (1.0f + st.y);
+  }
   // p (-lead - gH (x - mu)) = e (alpha + beta x)
-  const float beta = -gh * inv, alpha = (gh * st.z - lead) * inv;
-  const Base base(st.x);
-  if (__any_sync(kFullMask, base.far || lane_min(z) < kLowest)) {
-#pragma unroll
-    for (int i = 0; i < kRowElems; ++i) {
-      const float x = max_nan(z[i] - st.x, -200.0f);  // -inf: e is 0, and beta x finite
-      z[i] = ex2_approx(x * kLog2e) * fmaf(beta, x, alpha);
-    }
-  } else {
-    const float beta2 = beta * kLn2;
-    const F2 l2 = f2(kLog2e), neg_M = f2(base.neg_M), b2 = f2(beta2 * base.undo),
-             a2 = f2((alpha - beta2 * base.d) * base.undo);
-#pragma unroll
-    for (int i = 0; i < kRowElems; i += 2) {
-      const F2 y = fma2(f2(z[i], z[i + 1]), l2, neg_M);
-      float y0, y1;
-      split(y, y0, y1);
-      split(mul2(f2(ex2_approx(y0), ex2_approx(y1)), fma2(b2, y, a2)), z[i], z[i + 1]);
-    }
-  }
-  if (empty) {
-#pragma unroll
-    for (int i = 0; i < kRowElems; ++i) z[i] = 0.0f;
-  }
-  if (on) store_row(dz + c0, at, z);
-  sync();
-  if (!on || empty) return;
-  for (int j = lane; j <= k; j += lanes) {
-    const int64_t c = j < k ? (int64_t)tc[j] : code;
-    bool own_place = c >= c0 && c < c0 + len;
-    if (j == k)  // the given code, where it is none of the alternatives
-      for (int i = 0; i < k; ++i) own_place = own_place && (int64_t)tc[i] != code;
-    if (!own_place) continue;
-    float own = c == code ? gl : 0.0f, others = c == code ? 0.0f : gl;
+  __device__ __forceinline__ float beta() const { return -gh * inv; }
+  __device__ __forceinline__ float alpha() const { return (gh * st.z - lead) * inv; }
+};
+// The second writing of a place: alternative j, or (j = top_k) the given code where it
+// is none of the alternatives. Its loads can be made ahead.
+struct Special {
+  int64_t c;  // -1: none
+  float own, others, z;
+  template <typename T>
+  __device__ __forceinline__ Special(const LogProbsIn& in, const RowGrad& g, int64_t row, int j,
+                                     const T* __restrict__ p) {
+    const int k = in.top_k;
+    const int32_t* tc = in.top_codes + row * k;
+    const float* gt = in.g_top + row * k;
+    c = j < k ? (int64_t)tc[j] : j == k ? g.code : -1;
+    own = c == g.code ? g.gl : 0.0f;
+    others = c == g.code ? 0.0f : g.gl;
     for (int i = 0; i < k; ++i) {
+      if (j == k && (int64_t)tc[i] == c) c = -1;
       if (i == j) own += gt[i];
       else others += gt[i];
     }
-    const float x = to_f32(p[c]) - st.x;
-    const float pr = ex2_approx(x * kLog2e) * inv;
-    const float not_p = x == 0.0f ? st.y * inv : 1.0f - pr;
-    const float h = pr == 0.0f ? 0.0f : gh * pr * (x - st.z);
+    if (g.empty) c = -1;
+    z = c >= 0 ? to_f32(p[c]) : 0.0f;
+  }
+  template <typename T>
+  __device__ __forceinline__ void write(const RowGrad& g, T* __restrict__ dz) const {
+    const float x = z - g.st.x;
+    const float pr = ex2_approx(x * kLog2e) * g.inv;
+    const float not_p = x == 0.0f ? g.st.y * g.inv : 1.0f - pr;
+    const float h = pr == 0.0f ? 0.0f : g.gh * pr * (x - g.st.z);
     dz[c] = from_f32<T>(own * not_p - others * pr - h);
+  }
+};
+
+// e (alpha + beta x) of a lane's values, in place (far: Base does not hold); 0 at -inf.
+__device__ __forceinline__ void row_grad(float (&z)[kRowElems], bool far, float m, float alpha, float beta,
+                                         float neg_M, float a2, float b2) {
+  if (__any_sync(kFullMask, far || lane_min(z) < kLowest)) {
+#pragma unroll
+    for (int i = 0; i < kRowElems; ++i) {
+      const float x = max_nan(z[i] - m, -200.0f);  // e is 0, and beta x finite
+      z[i] = ex2_approx(x * kLog2e) * fmaf(beta, x, alpha);
+    }
+  } else {
+    const F2 l2 = f2(kLog2e), M2 = f2(neg_M), B = f2(b2), A = f2(a2);
+#pragma unroll
+    for (int i = 0; i < kRowElems; i += 2) {
+      const F2 y = fma2(f2(z[i], z[i + 1]), l2, M2);
+      float y0, y1;
+      split(y, y0, y1);
+      split(mul2(f2(ex2_approx(y0), ex2_approx(y1)), fma2(B, y, A)), z[i], z[i + 1]);
+    }
   }
 }
 
+// Rows of up to 512 codes, 32 to a warp: what a row costs besides its values is done
+// for 32 rows at once, a lane each; then L lanes a row go through the values of 32 / L
+// rows at a time.
 template <typename T, Mode M, bool SAME, int L>
 __global__ void __launch_bounds__(kGroupThreads, kRowThreadsSM / kGroupThreads)
     k_log_probs_bwd_group(int64_t rows, int C, const T* __restrict__ logits, int64_t stride, LogProbsIn in,
                           T* __restrict__ g_logits) {
   pdl_wait();
   pdl_trigger();
-  const int64_t mine = ((int64_t)blockIdx.x * kGroupThreads + threadIdx.x) / L;
-  const bool on = mine < rows;
-  const int64_t row = on ? mine : rows - 1;
-  T* dz = g_logits + row * C;
-  log_probs_grad<SAME>(row, C, 0, Deal<T, M>(C, L, threadIdx.x % L, dz), on, logits + row * stride, dz, in,
-                       [] { __syncwarp(); });
+  const int lane32 = threadIdx.x % 32, lane = lane32 % L;
+  const int64_t row0 = ((int64_t)blockIdx.x * kGroupThreads + threadIdx.x) / 32 * 32;
+  if (row0 >= rows) return;
+  const int64_t own = min(row0 + lane32, rows - 1);
+  const RowGrad g(in, own, C);
+  const Base base(g.st.x);
+  const float beta = g.beta(), alpha = g.alpha(), beta2 = beta * kLn2;
+  const float b2 = beta2 * base.undo, a2 = (alpha - beta2 * base.d) * base.undo;
+  const bool far = base.far && !g.empty;  // an empty row's values are not used
+#pragma unroll 1
+  for (int h = 0; h < L; ++h) {
+    const int from = h * (32 / L) + lane32 / L;
+    if (row0 + h * (32 / L) >= rows) break;
+    const int64_t row = min(row0 + from, rows - 1);
+    const bool on = row0 + from < rows;
+    const T* p = logits + row * stride;
+    T* dz = g_logits + row * C;
+    const Deal<T, M> at(C, L, lane, dz);
+    float z[kRowElems];
+    if constexpr (SAME) load_row(p, at, 0u, z);
+    else load_row_single(p, at, z);
+    auto of = [&](float v) { return __shfl_sync(kFullMask, v, from); };
+    const bool empty = __shfl_sync(kFullMask, g.empty, from);
+    row_grad(z, __shfl_sync(kFullMask, far, from), of(g.st.x), of(alpha), of(beta), of(base.neg_M), of(a2), of(b2));
+    if (empty) {
+#pragma unroll
+      for (int i = 0; i < kRowElems; ++i) z[i] = 0.0f;
+    }
+    if (on) store_row(dz, at, z);
+  }
+  __syncwarp();  // the second writing comes after the first
+  if (row0 + lane32 >= rows) return;
+  for (int j = 0; j <= in.top_k; ++j) {
+    const Special sp(in, g, own, j, logits + own * stride);
+    if (sp.c >= 0) sp.write(g, g_logits + own * C);
+  }
 }
 
+// Longer rows: W warps a stretch. `at` deals out the result's values (SAME: the
+// logits' lie alike).
 template <typename T, Mode M, bool SAME, int W>
 __global__ void __launch_bounds__(W * 32, kRowThreadsSM / (W * 32))
     k_log_probs_bwd_block(int64_t items, int64_t C, int parts, int part_len, const T* __restrict__ logits,
@@ -440,9 +480,29 @@ __global__ void __launch_bounds__(W * 32, kRowThreadsSM / (W * 32))
     const int64_t row = parts == 1 ? item : item / parts;
     const int c0 = (int)(item - row * parts) * part_len;
     const int len = (int)min((int64_t)part_len, C - c0);
+    const T* p = logits + row * stride;
     T* dz = g_logits + row * C;
-    log_probs_grad<SAME>(row, C, c0, Deal<T, M>(len, W * 32, threadIdx.x, dz + c0), true, logits + row * stride, dz,
-                         in, [] { __syncthreads(); });
+    const Deal<T, M> at(len, W * 32, threadIdx.x, dz + c0);
+    float z[kRowElems];
+    if constexpr (SAME) load_row(p + c0, at, 0u, z);
+    else load_row_single(p + c0, at, z);
+    const RowGrad g(in, row, C);
+    const Special sp(in, g, row, threadIdx.x <= in.top_k ? (int)threadIdx.x : in.top_k + 1, p);
+    const Base base(g.st.x);
+    const float beta = g.beta(), alpha = g.alpha(), beta2 = beta * kLn2;
+    row_grad(z, base.far && !g.empty, g.st.x, alpha, beta, base.neg_M, (alpha - beta2 * base.d) * base.undo,
+             beta2 * base.undo);
+    if (g.empty) {
+#pragma unroll
+      for (int i = 0; i < kRowElems; ++i) z[i] = 0.0f;
+    }
+    store_row(dz + c0, at, z);
+    __syncthreads();  // the second writing comes after the first
+    if (sp.c >= c0 && sp.c < c0 + len) sp.write(g, dz);
+    if (W == 1 && in.top_k == 32 && threadIdx.x == 0) {  // one place more than threads
+      const Special more(in, g, row, 32, p);
+      if (more.c >= c0 && more.c < c0 + len) more.write(g, dz);
+    }
   }
 }
 
@@ -547,7 +607,7 @@ extern "C" int gsb_code_log_probs_backward(int32_t dtype, int64_t rows, int64_t 
     if (plan.lanes > 0) {
       with_lanes(plan.lanes, [&](auto l) {
         constexpr int L = decltype(l)::value;
-        launch_pdl(k_log_probs_bwd_group<T, M, SAME, L>, grid1d(rows * L, kGroupThreads), kGroupThreads, 0, s, rows,
+        launch_pdl(k_log_probs_bwd_group<T, M, SAME, L>, grid1d(rows, kGroupThreads), kGroupThreads, 0, s, rows,
                    (int)codebook_rows, (const T*)logits, logits_stride, in, (T*)g_logits);
       });
     } else {
