@@ -51,60 +51,148 @@ __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&v)[V]
 
 // One thread per V values of the result and kLookupItems such pieces, a block's
 // width apart: stores of a warp are contiguous whatever the row's length, and the
-// loads of the pieces (code, then row) overlap. Bound by the stores: the table
-// and the codes of neighbouring threads come from L2 and L1.
+// loads of the pieces overlap. A block's codes and weights go through shared memory
+// (kStage; they are each wanted by every piece of a row) unless rows are so short that
+// there are too many of them. Bound by the stores: the table comes from L2 and L1.
 constexpr int kLookupItems = 4;
-template <typename T, typename O, int V>
+constexpr int kLookupPieces = 256 * kLookupItems;  // a block's
+constexpr int kLookupSlots = 2048;                 // that are staged, at most
+template <typename T, typename O, int V, bool kStage>
 __global__ void __launch_bounds__(256)
-    k_lookup(int64_t pieces, int bag, int64_t C, int nvec, FastDiv div_nvec, const T* __restrict__ table,
-             int64_t stride, Codes codes, const float* __restrict__ weights, float scale, O* __restrict__ out,
-             uint32_t* status) {
+    k_lookup(int64_t pieces, int bag, int64_t C, int nvec, FastDiv div_nvec,
+             const T* __restrict__ table, int64_t stride, Codes codes, const float* __restrict__ weights, float scale,
+             O* __restrict__ out, uint32_t* status) {
   pdl_wait();
   pdl_trigger();
-  const int64_t tile = (int64_t)blockIdx.x * (256 * kLookupItems);
+  __shared__ int2 s_slot[kStage ? kLookupSlots : 1];  // code (-1: none), weight
+  const int64_t tile = (int64_t)blockIdx.x * kLookupPieces;
   const int64_t row0 = tile / nvec;
   const int off0 = (int)(tile - row0 * nvec);
+  auto slot = [&](int64_t i) {
+    int64_t c = codes.at(i);
+    if (c >= C) {
+      bad_code(status, kSiteCode);
+      c = -1;
+    }
+    return make_int2(c < 0 ? -1 : (int)c, __float_as_int(weights ? weights[i] : 1.0f));
+  };
+  if (kStage) {
+    const int64_t last = min(tile + kLookupPieces, pieces) - 1;
+    const int n = (int)(last / nvec - row0 + 1) * bag;
+    for (int i = threadIdx.x; i < n; i += 256) s_slot[i] = slot(row0 * bag + i);
+    __syncthreads();
+  }
+  float acc[kLookupItems][V];
+  int r[kLookupItems], d[kLookupItems];
 #pragma unroll
   for (int k = 0; k < kLookupItems; ++k) {
-    const int local = off0 + k * 256 + (int)threadIdx.x;
-    if (tile + (local - off0) >= pieces) break;
-    const int r = fast_div(local, div_nvec);
-    const int64_t n = row0 + r;
-    const int d = (local - r * nvec) * V;
-    float acc[V];
+    const int local = min(off0 + k * 256 + (int)threadIdx.x, off0 + (int)min((int64_t)kLookupPieces, pieces - tile) - 1);
+    r[k] = fast_div(local, div_nvec);
+    d[k] = (local - r[k] * nvec) * V;
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-    for (int j = 0; j < bag; ++j) {
-      const int64_t c = codes.at(n * bag + j);
-      if (c < 0) continue;
-      if (c >= C) {
-        bad_code(status, kSiteCode);
-        continue;
-      }
-      const float w = weights ? weights[n * bag + j] : 1.0f;
-      Vec<V, T> t;
-      t.load(table + c * stride + d);
+    for (int i = 0; i < V; ++i) acc[k][i] = 0.0f;
+  }
+  for (int j = 0; j < bag; ++j) {
+    Vec<V, T> t[kLookupItems];
+    float w[kLookupItems];
 #pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] = fmaf(w, t.v[i], acc[i]);
+    for (int k = 0; k < kLookupItems; ++k) {
+      const int2 s = kStage ? s_slot[r[k] * bag + j] : slot((row0 + r[k]) * bag + j);
+      w[k] = __int_as_float(s.y);
+#pragma unroll
+      for (int i = 0; i < V; ++i) t[k].v[i] = 0.0f;
+      if (s.x >= 0) t[k].load(table + s.x * stride + d[k]);
+      else w[k] = 0.0f;  // an empty slot adds nothing, whatever its weight is
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] *= scale;
-    store_vec<V>(out + (tile + (local - off0)) * V, acc);
+    for (int k = 0; k < kLookupItems; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[k][i] = fmaf(w[k], t[k].v[i], acc[k][i]);
+  }
+#pragma unroll
+  for (int k = 0; k < kLookupItems; ++k) {
+    const int64_t piece = tile + k * 256 + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[k][i] *= scale;
+    if (piece < pieces) store_vec<V>(out + piece * V, acc[k]);
   }
 }
 
-// Sort keys: the code, or C for an empty slot (sorted behind every code).
-__global__ void __launch_bounds__(256)
-    k_code_keys(int64_t n, int64_t C, Codes codes, uint32_t* __restrict__ keys, uint32_t* __restrict__ vals,
-                uint32_t* status) {
-  pdl_wait();
-  pdl_trigger();
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n) return;
+// Sort key of slot i: its code, or C for an empty one (sorted behind every code).
+__device__ __forceinline__ uint32_t code_key(const Codes& codes, int64_t i, int64_t C, uint32_t* status) {
   const int64_t c = codes.at(i);
   if (c >= C) bad_code(status, kSiteCode);
-  keys[i] = (c < 0 || c >= C) ? (uint32_t)C : (uint32_t)c;
-  vals[i] = (uint32_t)i;
+  return (c < 0 || c >= C) ? (uint32_t)C : (uint32_t)c;
+}
+// Zeroes the bytes of the table's gradient (rows that no code names stay 0).
+__device__ __forceinline__ void zero_words(uint32_t* to, int64_t bytes) {
+  const int64_t words = bytes / 4, step = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < words; i += step) to[i] = 0u;
+  if (bytes % 4 != 0 && blockIdx.x == 0 && threadIdx.x == 0) reinterpret_cast<uint16_t*>(to)[words * 2] = 0;
+}
+
+// Keys and slots for the sort, and the counts of the keys' 8-bit digits that it needs.
+constexpr int kKeyItems = 8;
+__global__ void __launch_bounds__(256)
+    k_code_keys(int64_t n, int64_t C, int passes, Codes codes, uint32_t* __restrict__ keys,
+                uint32_t* __restrict__ vals, uint32_t* __restrict__ digits, uint32_t* __restrict__ zero,
+                int64_t zero_bytes, uint32_t* status) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ uint32_t s_digits[4][kRadix];
+  for (int i = threadIdx.x; i < passes * kRadix; i += 256) (&s_digits[0][0])[i] = 0;
+  __syncthreads();
+  for (int64_t i0 = (int64_t)blockIdx.x * 256 * kKeyItems; i0 < n; i0 += (int64_t)gridDim.x * 256 * kKeyItems) {
+#pragma unroll
+    for (int k = 0; k < kKeyItems; ++k) {
+      const int64_t i = i0 + k * 256 + threadIdx.x;
+      if (i >= n) break;
+      const uint32_t key = code_key(codes, i, C, status);
+      keys[i] = key;
+      vals[i] = (uint32_t)i;
+      for (int p = 0; p < passes; ++p) atomicAdd(&s_digits[p][(key >> (8 * p)) & (kRadix - 1)], 1u);
+    }
+  }
+  zero_words(zero, zero_bytes);
+  __syncthreads();
+  for (int i = threadIdx.x; i < passes * kRadix; i += 256) {
+    const uint32_t v = (&s_digits[0][0])[i];
+    if (v) atomicAdd(&digits[i], v);
+  }
+}
+
+// Few slots: one block sorts them (a bitonic network on key and slot together, so
+// that equal keys keep their order), in one launch instead of four or five.
+constexpr int kFewSlots = 4096;
+__global__ void __launch_bounds__(1024)
+    k_sort_few(int n, int64_t C, Codes codes, uint32_t* __restrict__ keys, uint32_t* __restrict__ vals,
+               uint32_t* __restrict__ zero, int64_t zero_bytes, uint32_t* status) {
+  pdl_wait();
+  pdl_trigger();
+  if (blockIdx.x > 0) {  // the others zero the gradient
+    zero_words(zero, zero_bytes);
+    return;
+  }
+  __shared__ uint64_t s_key[kFewSlots];
+  int size = 32;
+  while (size < n) size *= 2;
+  for (int i = threadIdx.x; i < size; i += 1024)
+    s_key[i] = i < n ? ((uint64_t)code_key(codes, i, C, status) << 32) | (uint32_t)i : ~uint64_t(0);
+  zero_words(zero, zero_bytes);
+  __syncthreads();
+  for (int span = 2; span <= size; span *= 2)
+    for (int gap = span / 2; gap > 0; gap /= 2) {
+      for (int i = threadIdx.x; i < size / 2; i += 1024) {
+        const int lo = 2 * i - (i & (gap - 1)), hi = lo + gap;
+        const uint64_t x = s_key[lo], y = s_key[hi];
+        if ((x > y) == ((lo & span) == 0)) s_key[lo] = y, s_key[hi] = x;
+      }
+      __syncthreads();
+    }
+  for (int i = threadIdx.x; i < n; i += 1024) {
+    keys[i] = (uint32_t)(s_key[i] >> 32);
+    vals[i] = (uint32_t)s_key[i];
+  }
 }
 
 // Sums of the sorted entries, run by run (a run: the entries of one code).
@@ -129,7 +217,7 @@ template <int GL>
 constexpr int run_block_entries() { return run_entries<GL>() * (256 / GL); }
 
 template <typename T, typename O, int V, int GL, int R, bool WGRAD>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, WGRAD ? 1 : 4)
     k_run_sums(int n, int bag, FastDiv div_bag, int C, int dim, const uint32_t* __restrict__ keys,
                const uint32_t* __restrict__ vals, const float* __restrict__ weights, float scale,
                const O* __restrict__ g, const T* __restrict__ table, int64_t stride, T* __restrict__ g_table,
@@ -137,7 +225,9 @@ __global__ void __launch_bounds__(256)
   pdl_wait();
   pdl_trigger();
   constexpr int NG = 256 / GL, E = run_entries<GL>(), L = run_block_entries<GL>(), W = GL * V * R;
-  constexpr int U = WGRAD ? 2 : 4;  // entries whose loads are in flight together
+  // Entries whose loads are in flight together. Two of them and four blocks an SM took 56
+  // us where four and two took 61 (2^20 x 48 fp32); with WGRAD registers come first.
+  constexpr int U = 2;
   __shared__ uint32_t s_key[L + 2];  // the entries' keys, with the neighbours' on either side
   __shared__ uint32_t s_val[L];
   __shared__ __align__(16) float s_part[2][NG][W];
@@ -304,13 +394,19 @@ __global__ void __launch_bounds__(256)
   if (end >= n) return;
   const uint32_t key = keys[end - 1];
   if (key >= (uint32_t)C || keys[end] != key || (b0 > 0 && keys[b0 - 1] == key)) return;
-  int64_t lo = end, hi = n;  // first entry behind the run
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (keys[mid] <= key) lo = mid + 1;
-    else hi = mid;
+  // The blocks after this one that begin with the same code, 256 looked at at a time.
+  __shared__ int s_heads;
+  int64_t heads = 0;
+  for (bool more = true; more;) {
+    if (threadIdx.x == 0) s_heads = 256;
+    __syncthreads();
+    const int64_t at = end + (heads + threadIdx.x) * block_entries;
+    if (at >= n || keys[at] != key) atomicMin(&s_heads, (int)threadIdx.x);
+    __syncthreads();
+    heads += s_heads;
+    more = s_heads == 256;
+    __syncthreads();
   }
-  const int64_t heads = (lo - 1) / block_entries - blockIdx.x;
   const int cols = min(dim, 256), ways = 256 / cols;
   const int way = threadIdx.x / cols, col = threadIdx.x - way * cols;
   for (int d0 = 0; d0 < dim; d0 += cols) {
@@ -319,6 +415,7 @@ __global__ void __launch_bounds__(256)
     if (way < ways && d < dim) {
       const float* p = parts + (int64_t)blockIdx.x * 2 * dim + d;
       if (way == 0) acc = p[dim];
+#pragma unroll 4
       for (int64_t h = 1 + way; h <= heads; h += ways) acc += p[h * 2 * dim];
     }
     s_sum[threadIdx.x] = acc;
@@ -451,14 +548,17 @@ extern "C" int gsb_codebook_forward(int32_t table_dtype, int32_t out_dtype, int6
   const int so = dtype_bytes(out_dtype), st = dtype_bytes(table_dtype);
   const int V = dim % 4 == 0 && table_stride % 4 == 0 && aligned_to(table, 4 * st) && aligned_to(out, 4 * so) ? 4 : 1;
   const int64_t pieces = rows * (dim / V);
-  const int64_t blocks = (pieces + 256 * kLookupItems - 1) / (256 * kLookupItems);
+  const int64_t blocks = (pieces + kLookupPieces - 1) / kLookupPieces;
   if (blocks >= (int64_t(1) << 31)) return GSB_ERR_CAPACITY;
   with_dtypes(table_dtype, out_dtype, [&](auto t, auto o) {
       using T = decltype(t);
       using O = decltype(o);
-      launch_pdl(V == 4 ? k_lookup<T, O, 4> : k_lookup<T, O, 1>, (unsigned)blocks, 256, 0,
-                 static_cast<cudaStream_t>(stream), pieces, bag, codebook_rows, dim / V,
-                 make_fast_div((uint32_t)(dim / V)), (const T*)table, table_stride, cd, weights, scale, (O*)out, status);
+      const bool stage = (int64_t)(kLookupPieces / (dim / V) + 2) * bag <= kLookupSlots;
+      auto kernel = V == 4 ? (stage ? k_lookup<T, O, 4, true> : k_lookup<T, O, 4, false>)
+                           : (stage ? k_lookup<T, O, 1, true> : k_lookup<T, O, 1, false>);
+      launch_pdl(kernel, (unsigned)blocks, 256, 0, static_cast<cudaStream_t>(stream), pieces, bag,
+                 codebook_rows, dim / V, make_fast_div((uint32_t)(dim / V)),
+                 (const T*)table, table_stride, cd, weights, scale, (O*)out, status);
   });
   note_launches(1);
   return cuda_status(cudaGetLastError());
@@ -496,11 +596,23 @@ extern "C" int gsb_codebook_backward(int32_t table_dtype, int32_t out_dtype, int
       return GSB_ERR_WORKSPACE;
     Carver ws(workspace);
     const BackwardScratch b = carve(ws, slots, dim);
-    if (cudaMemsetAsync(g_table, 0, (size_t)codebook_rows * dim * dtype_bytes(table_dtype), s) != cudaSuccess)
-      return GSB_ERR_CUDA;  // the rows that no code names
-    launch_pdl(k_code_keys, grid1d(slots, 256), 256, 0, s, slots, codebook_rows, cd, b.keys, b.vals, status);
-    e = radix_sort_pairs(ws, b.keys, b.vals, b.keys_s, b.vals_s, slots, 0, bits_for(codebook_rows), status, s, false);
-    if (e != cudaSuccess) return GSB_ERR_CUDA;
+    const int64_t table_bytes = codebook_rows * dim * dtype_bytes(table_dtype);
+    const int zero_blocks = (int)std::min<int64_t>(148 * 8, (table_bytes + (1 << 14) - 1) >> 14);
+    if (slots <= kFewSlots) {
+      launch_pdl(k_sort_few, zero_blocks, 1024, 0, s, (int)slots, codebook_rows, cd, b.keys_s, b.vals_s,
+                 (uint32_t*)g_table, table_bytes, status);
+      note_launches(1);
+    } else {
+      const int bits = bits_for(codebook_rows);
+      const ZeroRegion zero = radix_sort_zero_region(ws, slots, 0, bits, true);  // begins with the digits' counts
+      if (cudaMemsetAsync(zero.ptr, 0, zero.words * sizeof(uint32_t), s) != cudaSuccess) return GSB_ERR_CUDA;
+      const int blocks = std::max(zero_blocks, (int)std::min<int64_t>(148 * 8, grid1d(slots, 256 * kKeyItems)));
+      launch_pdl(k_code_keys, blocks, 256, 0, s, slots, codebook_rows, sort_passes(0, bits), cd, b.keys, b.vals,
+                 zero.ptr, (uint32_t*)g_table, table_bytes, status);
+      note_launches(1);
+      e = radix_sort_pairs(ws, b.keys, b.vals, b.keys_s, b.vals_s, slots, 0, bits, status, s, true, zero.ptr);
+      if (e != cudaSuccess) return GSB_ERR_CUDA;
+    }
     const int so = dtype_bytes(out_dtype), st = dtype_bytes(table_dtype);
     const bool vec = dim % 4 == 0 && aligned_to(grad_out, 4 * so) && aligned_to(g_table, 4 * st) &&
                      (!g_weights || (table_stride % 4 == 0 && aligned_to(table, 4 * st)));
@@ -523,7 +635,7 @@ extern "C" int gsb_codebook_backward(int32_t table_dtype, int32_t out_dtype, int
           launch_pdl(k_run_parts<T>, grid.x - 1, 256, 0, s, (int)slots, (int)codebook_rows, dim, block_entries,
                      (const uint32_t*)b.keys_s, scale, (const float*)b.parts, (T*)g_table);
     });
-    note_launches(grid.x > 1 ? 3 : 2);
+    note_launches(grid.x > 1 ? 2 : 1);
     if (fused) g_weights = nullptr;  // done
   }
   if (g_weights) {
