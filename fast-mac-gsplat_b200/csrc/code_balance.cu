@@ -222,20 +222,21 @@ __global__ void __launch_bounds__(256)
 }
 
 // dz_c = g coef p_c ((n_c - n_a) - dr); `at` deals out the result's values (SAME: the
-// logits' lie alike).
+// logits' lie alike), p and dz are their place 0, that of code -shift.
 template <bool SAME, typename T, Mode M>
-__device__ __forceinline__ void balance_grad(float k, float4 st, const Deal<T, M>& at, bool on,
+__device__ __forceinline__ void balance_grad(float k, float4 st, const Deal<T, M>& at, int shift, bool on,
                                              const T* __restrict__ p, const Counts& counts, T* __restrict__ dz) {
   float z[kRowElems];
-  if constexpr (SAME) load_row(p, at, 0u, z);
+  if constexpr (SAME) load_row(p, at, z);
   else load_row_single(p, at, z);
+  const Counts::Offsets off(counts, shift);
   const Base base(st.x);
   if (__any_sync(kFullMask, base.far)) {
     const float f = k * st.y;
 #pragma unroll
     for (int i = 0; i < kRowElems; i += 4) {
       float n[4];
-      counts.four(at, i, n);
+      counts.four(at, shift, off, i, n);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float e = ex2_approx((z[i + j] - st.x) * kLog2e);
@@ -248,9 +249,9 @@ __device__ __forceinline__ void balance_grad(float k, float4 st, const Deal<T, M
              f = f2(k * st.y * base.undo);
 #pragma unroll
     for (int i = 0; i < kRowElems; i += 4) {
-      if (!at.any(i)) continue;
+      if (!at.full && at.place(i) - at.lane * Deal<T, M>::VEC >= at.hi) continue;  // no lane has any
       float n[4];
-      counts.four(at, i, n);
+      counts.four(at, shift, off, i, n);
 #pragma unroll
       for (int j = 0; j < 4; j += 2) {
         float y0, y1;
@@ -275,8 +276,9 @@ __global__ void __launch_bounds__(kGroupThreads, kRowThreadsSM / kGroupThreads)
   const bool on = mine < rows;
   const int64_t row = on ? mine : rows - 1;
   T* dz = g_logits + row * C;
-  balance_grad<SAME>(k, stats[row], Deal<T, M>(C, L, threadIdx.x % L, dz), on, logits + row * stride,
-                     counts_of(state, C), dz);
+  const int shift = shift_of<T, M>(dz);
+  balance_grad<SAME>(k, stats[row], Deal<T, M>(shift, C + shift, L, threadIdx.x % L), shift, on,
+                     logits + row * stride - shift, counts_of(state, C), dz - shift);
 }
 
 template <typename T, Mode M, bool SAME, int W>
@@ -289,11 +291,12 @@ __global__ void __launch_bounds__(W * 32, kRowThreadsSM / (W * 32))
   const float k = *g_loss * state[0];
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int64_t row = parts == 1 ? item : item / parts;
-    const int c0 = (int)(item - row * parts) * part_len;
-    const int len = (int)min((int64_t)part_len, C - c0);
-    T* dz = g_logits + row * C + c0;
-    balance_grad<SAME>(k, stats[row], Deal<T, M>(len, W * 32, threadIdx.x, dz), true, logits + row * stride + c0,
-                       counts_of(state, C).from(c0), dz);
+    T* dz = g_logits + row * C;
+    const int shift = shift_of<T, M>(dz), part = (int)(item - row * parts);
+    const int c0 = part * part_len;  // of place 0, but for the shift
+    const int hi = (int)min((int64_t)part_len, C + shift - c0), lo = part == 0 ? shift : 0;
+    balance_grad<SAME>(k, stats[row], Deal<T, M>(lo, hi, W * 32, threadIdx.x), shift, true,
+                       logits + row * stride + c0 - shift, counts_of(state, C).from(c0), dz + c0 - shift);
   }
 }
 
@@ -418,7 +421,7 @@ extern "C" int gsb_code_balance_backward(int32_t dtype, int64_t rows, int64_t co
     using T = decltype(t);
     constexpr Mode M = decltype(m)::value;
     constexpr bool SAME = decltype(same)::value;
-    const RowPlan plan = row_plan(rows, codebook_rows, M == Mode::kShifted);
+    const RowPlan plan = row_plan(rows, codebook_rows, M == Mode::kShifted, Deal<T, M>::VEC);
     if (plan.lanes > 0) {
       with_lanes(plan.lanes, [&](auto l) {
         constexpr int L = decltype(l)::value;

@@ -447,10 +447,11 @@ __global__ void __launch_bounds__(kGroupThreads, kRowThreadsSM / kGroupThreads)
     const bool on = row0 + from < rows;
     const T* p = logits + row * stride;
     T* dz = g_logits + row * C;
-    const Deal<T, M> at(C, L, lane, dz);
+    const int shift = shift_of<T, M>(dz);
+    const Deal<T, M> at(shift, C + shift, L, lane);
     float z[kRowElems];
-    if constexpr (SAME) load_row(p, at, 0u, z);
-    else load_row_single(p, at, z);
+    if constexpr (SAME) load_row(p - shift, at, z);
+    else load_row_single(p - shift, at, z);
     auto of = [&](float v) { return __shfl_sync(kFullMask, v, from); };
     const bool empty = __shfl_sync(kFullMask, g.empty, from);
     row_grad(z, __shfl_sync(kFullMask, far, from), of(g.st.x), of(alpha), of(beta), of(base.neg_M), of(a2), of(b2));
@@ -458,7 +459,7 @@ __global__ void __launch_bounds__(kGroupThreads, kRowThreadsSM / kGroupThreads)
 #pragma unroll
       for (int i = 0; i < kRowElems; ++i) z[i] = 0.0f;
     }
-    if (on) store_row(dz, at, z);
+    if (on) store_row(dz - shift, at, z);
   }
   __syncwarp();  // the second writing comes after the first
   if (row0 + lane32 >= rows) return;
@@ -468,8 +469,7 @@ __global__ void __launch_bounds__(kGroupThreads, kRowThreadsSM / kGroupThreads)
   }
 }
 
-// Longer rows: W warps a stretch. `at` deals out the result's values (SAME: the
-// logits' lie alike).
+// Longer rows: W warps a stretch of the result (SAME: the logits' rows lie alike).
 template <typename T, Mode M, bool SAME, int W>
 __global__ void __launch_bounds__(W * 32, kRowThreadsSM / (W * 32))
     k_log_probs_bwd_block(int64_t items, int64_t C, int parts, int part_len, const T* __restrict__ logits,
@@ -478,13 +478,14 @@ __global__ void __launch_bounds__(W * 32, kRowThreadsSM / (W * 32))
   pdl_trigger();
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int64_t row = parts == 1 ? item : item / parts;
-    const int c0 = (int)(item - row * parts) * part_len;
-    const int len = (int)min((int64_t)part_len, C - c0);
     const T* p = logits + row * stride;
     T* dz = g_logits + row * C;
-    const Deal<T, M> at(len, W * 32, threadIdx.x, dz + c0);
+    const int shift = shift_of<T, M>(dz), part = (int)(item - row * parts);
+    const int c0 = part * part_len - shift;  // the code of place 0
+    const int hi = (int)min((int64_t)part_len, C - c0), lo = part == 0 ? shift : 0;
+    const Deal<T, M> at(lo, hi, W * 32, threadIdx.x);
     float z[kRowElems];
-    if constexpr (SAME) load_row(p + c0, at, 0u, z);
+    if constexpr (SAME) load_row(p + c0, at, z);
     else load_row_single(p + c0, at, z);
     const RowGrad g(in, row, C);
     const Special sp(in, g, row, threadIdx.x <= in.top_k ? (int)threadIdx.x : in.top_k + 1, p);
@@ -498,10 +499,10 @@ __global__ void __launch_bounds__(W * 32, kRowThreadsSM / (W * 32))
     }
     store_row(dz + c0, at, z);
     __syncthreads();  // the second writing comes after the first
-    if (sp.c >= c0 && sp.c < c0 + len) sp.write(g, dz);
+    if (sp.c >= max(c0, 0) && sp.c < c0 + hi) sp.write(g, dz);
     if (W == 1 && in.top_k == 32 && threadIdx.x == 0) {  // one place more than threads
       const Special more(in, g, row, 32, p);
-      if (more.c >= c0 && more.c < c0 + len) more.write(g, dz);
+      if (more.c >= max(c0, 0) && more.c < c0 + hi) more.write(g, dz);
     }
   }
 }
@@ -603,7 +604,7 @@ extern "C" int gsb_code_log_probs_backward(int32_t dtype, int64_t rows, int64_t 
     using T = decltype(t);
     constexpr Mode M = decltype(m)::value;
     constexpr bool SAME = decltype(same)::value;
-    const RowPlan plan = row_plan(rows, codebook_rows, M == Mode::kShifted);
+    const RowPlan plan = row_plan(rows, codebook_rows, M == Mode::kShifted, Deal<T, M>::VEC);
     if (plan.lanes > 0) {
       with_lanes(plan.lanes, [&](auto l) {
         constexpr int L = decltype(l)::value;

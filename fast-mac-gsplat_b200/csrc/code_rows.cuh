@@ -33,7 +33,6 @@ constexpr int kGroupMaxLanes = 16;     // lanes a row, several rows a warp
 constexpr int kGroupMaxCodes = kGroupMaxLanes * kRowElems;
 constexpr int kBlockMaxWarps = 8;
 constexpr int kRowThreadsSM = 1024;     // threads an SM that registers are kept for (64 each)
-constexpr int kBlockMaxCodes = kBlockMaxWarps * 32 * kRowElems;
 
 __device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
 __device__ __forceinline__ float quiet_nan() { return __int_as_float(0x7fc00000); }
@@ -74,69 +73,69 @@ __device__ __forceinline__ uint32_t nan_bits<__nv_bfloat16>() { return 0x7fc07fc
 template <>
 __device__ __forceinline__ uint32_t nan_bits<__half>() { return 0x7e007e00u; }
 
-// How a stretch of len values of a row is dealt out to `lanes` lanes: lane l's value
-// k has the index (k / VEC lanes + l) VEC + k % VEC - shift. VEC is 1, or the values
-// of a 16-byte piece. shift: values between the 16-byte boundary before the stretch
-// and its start (Mode::kShifted alone), so that pieces lie on boundaries whatever
-// the row's length; the pieces at its ends are read and written by the value.
+// How a stretch of a row is dealt out to `lanes` lanes: lane l's value k has the
+// place (k / VEC lanes + l) VEC + k % VEC. VEC is 1, or the values of a 16-byte piece.
+// Where rows begin between 16-byte boundaries (Mode::kShifted) places count from the
+// boundary before the row's first value, `shift` values before it, so that pieces lie
+// on boundaries whatever the row's length. Places lo .. hi - 1 hold values; `full`:
+// the first nv pieces of every lane are whole and the others empty, and nothing else is
+// checked.
 enum class Mode { kSingle, kWide, kShifted };
 template <typename T, Mode M>
 struct Deal {
   static constexpr int VEC = M == Mode::kSingle ? 1 : wide_of<T>();
-  static constexpr bool kShift = M == Mode::kShifted;
-  int len, lanes, lane, shift;
-  __device__ __forceinline__ Deal(int len, int lanes, int lane, const T* p)
-      : len(len), lanes(lanes), lane(lane),
-        shift(kShift ? (int)(reinterpret_cast<uintptr_t>(p) % 16 / sizeof(T)) : 0) {}
-  __device__ __forceinline__ int index(int k) const { return ((k / VEC) * lanes + lane) * VEC + k % VEC - shift; }
-  __device__ __forceinline__ bool has(int c) const { return (!kShift || c >= 0) && c < len; }
-  __device__ __forceinline__ bool whole(int c) const { return (!kShift || c >= 0) && c + VEC <= len; }
-  // False if no lane has anything of its values k, ... of a piece (the same for all lanes).
-  __device__ __forceinline__ bool any(int k) const { return (k / VEC) * lanes * VEC - shift < len; }
-  // Whether all lanes have all of the values k .. k + 3.
-  __device__ __forceinline__ bool all(int k) const {
-    const int last = VEC == 1 ? k + 3 : k / VEC;  // of four values k, ...
-    return (last + 1) * lanes * VEC - shift <= len && (!kShift || k >= VEC || shift == 0);
+  int lo, hi, lanes, lane, nv;
+  bool full;
+  __device__ __forceinline__ Deal(int lo_, int hi_, int lanes_, int lane_)
+      : lo(lo_), hi(hi_), lanes(lanes_), lane(lane_), nv(hi_ / (lanes_ * VEC)) {
+    full = lo == 0 && hi == nv * lanes * VEC;
   }
-  // The lane and place of index c.
-  __device__ __forceinline__ int lane_of(int c) const { return (c + shift) / VEC % lanes; }
-  __device__ __forceinline__ int place_of(int c) const {
-    return (c + shift) / VEC / lanes * VEC + (c + shift) % VEC;
-  }
+  __device__ __forceinline__ int place(int k) const { return ((k / VEC) * lanes + lane) * VEC + k % VEC; }
+  __device__ __forceinline__ bool has(int c) const { return (M != Mode::kShifted || c >= lo) && c < hi; }
+  __device__ __forceinline__ bool whole(int c) const { return (M != Mode::kShifted || c >= lo) && c + VEC <= hi; }
+  __device__ __forceinline__ bool ragged(int c) const { return c + VEC > lo && c < hi && !whole(c); }
 };
-
-// Reads a lane's values; `fill` (the bits of a word of them) where there is none.
+// Values between the 16-byte boundary before p and p.
 template <typename T, Mode M>
-__device__ __forceinline__ void load_row(const T* __restrict__ p, const Deal<T, M>& at, uint32_t fill,
-                                         float (&z)[kRowElems]) {
+__device__ __forceinline__ int shift_of(const T* p) {
+  return M == Mode::kShifted ? (int)(reinterpret_cast<uintptr_t>(p) % 16 / sizeof(T)) : 0;
+}
+
+// Reads a lane's values (p: place 0); 0 where there is none.
+template <typename T, Mode M>
+__device__ __forceinline__ void load_row(const T* __restrict__ p, const Deal<T, M>& at, float (&z)[kRowElems]) {
   constexpr int VEC = Deal<T, M>::VEC;
   if constexpr (VEC == 1) {
     static_assert(sizeof(T) == 4, "values of two bytes are read in pieces");
 #pragma unroll
     for (int k = 0; k < kRowElems; ++k) {
-      const int c = at.index(k);
-      z[k] = __uint_as_float(fill);
-      if (c < at.len) z[k] = p[c];
+      const int c = at.place(k);
+      z[k] = 0.0f;
+      if (c < at.hi) z[k] = p[c];
     }
   } else {
     constexpr int NV = kRowElems / VEC;
     uint4 q[NV];
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int c = at.index(v * VEC);
-      q[v] = make_uint4(fill, fill, fill, fill);
-      if (at.whole(c)) q[v] = *reinterpret_cast<const uint4*>(p + c);
-    }
-    if (at.shift != 0 || at.len % VEC != 0) {
+    if (at.full) {
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const int c = at.index(v * VEC);
-        if (c + VEC > 0 && c < at.len && !at.whole(c)) {
-          T e[VEC];
-          *reinterpret_cast<uint4*>(e) = q[v];
+        q[v] = make_uint4(0u, 0u, 0u, 0u);
+        if (v < at.nv) q[v] = *reinterpret_cast<const uint4*>(p + at.place(v * VEC));
+      }
+    } else {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i)
+      for (int v = 0; v < NV; ++v) {
+        const int c = at.place(v * VEC);
+        q[v] = make_uint4(0u, 0u, 0u, 0u);
+        if (at.whole(c)) {
+          q[v] = *reinterpret_cast<const uint4*>(p + c);
+        } else if (M == Mode::kShifted && at.ragged(c)) {
+          T e[VEC];
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            e[i] = from_f32<T>(0.0f);
             if (at.has(c + i)) e[i] = p[c + i];
+          }
           q[v] = *reinterpret_cast<const uint4*>(e);
         }
       }
@@ -157,19 +156,18 @@ __device__ __forceinline__ void load_row_single(const T* __restrict__ p, const D
                                                 float (&z)[kRowElems]) {
   constexpr int VEC = Deal<T, M>::VEC;
   T q[kRowElems];
+  if (at.full) {
 #pragma unroll
-  for (int v = 0; v < kRowElems / VEC; ++v) {
-    const int c = at.index(v * VEC);
-    if (at.whole(c)) {
-      const T* pc = p + c;
+    for (int k = 0; k < kRowElems; ++k) {
+      q[k] = from_f32<T>(0.0f);
+      if (k / VEC < at.nv) q[k] = p[at.place(k)];
+    }
+  } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) q[v * VEC + i] = pc[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        q[v * VEC + i] = from_f32<T>(0.0f);
-        if (at.has(c + i)) q[v * VEC + i] = p[c + i];
-      }
+    for (int k = 0; k < kRowElems; ++k) {
+      const int c = at.place(k);
+      q[k] = from_f32<T>(0.0f);
+      if (at.has(c)) q[k] = p[c];
     }
   }
 #pragma unroll
@@ -183,22 +181,31 @@ __device__ __forceinline__ void store_row(T* __restrict__ p, const Deal<T, M>& a
   if constexpr (VEC == 1) {
 #pragma unroll
     for (int k = 0; k < kRowElems; ++k) {
-      const int c = at.index(k);
-      if (c < at.len) p[c] = from_f32<T>(d[k]);
+      const int c = at.place(k);
+      if (c < at.hi) p[c] = from_f32<T>(d[k]);
     }
   } else {
-#pragma unroll
-    for (int v = 0; v < kRowElems / VEC; ++v) {
-      const int c = at.index(v * VEC);
+    auto piece = [&](int v) {
       T e[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) e[i] = from_f32<T>(d[v * VEC + i]);
-      if (at.whole(c)) {
-        *reinterpret_cast<uint4*>(p + c) = *reinterpret_cast<const uint4*>(e);
-      } else if (c + VEC > 0 && c < at.len) {
+      return *reinterpret_cast<const uint4*>(e);
+    };
+    if (at.full) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          if (at.has(c + i)) p[c + i] = e[i];
+      for (int v = 0; v < kRowElems / VEC; ++v)
+        if (v < at.nv) *reinterpret_cast<uint4*>(p + at.place(v * VEC)) = piece(v);
+    } else {
+#pragma unroll
+      for (int v = 0; v < kRowElems / VEC; ++v) {
+        const int c = at.place(v * VEC);
+        if (at.whole(c)) {
+          *reinterpret_cast<uint4*>(p + c) = piece(v);
+        } else if (M == Mode::kShifted && at.ragged(c)) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            if (at.has(c + i)) p[c + i] = from_f32<T>(d[v * VEC + i]);
+        }
       }
     }
   }
@@ -213,33 +220,44 @@ struct Counts {
   int64_t eights;  // codes / 8, rounded up
   // Of the codes from c0 on, a multiple of 8.
   __device__ __forceinline__ Counts from(int64_t c0) const { return Counts{by_code + c0, by_eight + c0 / 8, eights}; }
-  // Those of a lane's values k .. k + 3; 0 where it has none.
+  // Where the count of value j of a piece is in by_eight, relative to that of the first
+  // 8-aligned code of the piece: code 8 q + j - shift has the same residue modulo 8 for
+  // every q.
+  struct Offsets {
+    int of[8];
+    __device__ __forceinline__ Offsets(const Counts& counts, int shift) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) of[j] = ((j - shift) & 7) * (int)counts.eights - (j < shift ? 1 : 0);
+    }
+  };
+  // Those of a lane's values k .. k + 3, place 0 being code -shift; 0 where it has none.
   template <typename T, Mode M>
-  __device__ __forceinline__ void four(const Deal<T, M>& at, int k, float (&n)[4]) const {
-    const int c = at.index(k);
+  __device__ __forceinline__ void four(const Deal<T, M>& at, int shift, const Offsets& off, int k,
+                                       float (&n)[4]) const {
+    const int c = at.place(k);
     if constexpr (M == Mode::kWide) {
-      const float4 q = c < at.len ? *reinterpret_cast<const float4*>(by_code + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 q = c < at.hi ? *reinterpret_cast<const float4*>(by_code + c)
+                                            : make_float4(0.f, 0.f, 0.f, 0.f);
       n[0] = q.x, n[1] = q.y, n[2] = q.z, n[3] = q.w;
     } else if constexpr (M == Mode::kShifted) {
       static_assert(Deal<T, M>::VEC == 8, "values of two bytes");
-      // The same residue modulo 8 in every lane: c + i = 8 q + j - shift.
-      const int q = (c - k % 8 + at.shift) >> 3;
-      if (at.whole(c - k % 8)) {
-        const float* p = by_eight + q;
+      const int first = c - k % 8;  // the piece's
+      const bool whole = at.whole(first);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = k % 8 + i;
-          n[i] = p[((j - at.shift) & 7) * eights - (j < at.shift ? 1 : 0)];
-        }
-      } else {
+      for (int i = 0; i < 4; ++i) {
+        n[i] = 0.0f;
+        if (whole) n[i] = by_eight[first / 8 + off.of[k % 8 + i]];
+      }
+      if (!at.full && at.ragged(first)) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) n[i] = at.has(c + i) ? by_code[c + i] : 0.0f;
+        for (int i = 0; i < 4; ++i)
+          if (at.has(c + i)) n[i] = by_code[c + i - shift];
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int ci = at.index(k + i);
-        n[i] = ci < at.len ? by_code[ci] : 0.0f;
+        const int ci = at.place(k + i);
+        n[i] = ci < at.hi ? by_code[ci] : 0.0f;
       }
     }
   }
@@ -350,31 +368,31 @@ constexpr float kLn2 = 0.6931471805599453f;
 // Below this z log2 e may be -inf, and its product with e = 0 NaN.
 constexpr float kLowest = -1e38f;
 
-// How the rows of a call are taken: `lanes` a row (kGroupMaxLanes or fewer: rows
-// side by side in a warp), else warps per stretch and stretches per row.
+// How the backward takes the rows of a call: `lanes` a row (kGroupMaxLanes or fewer:
+// rows side by side in a warp), else `warps` per stretch of part_len places (whole
+// pieces of all their lanes), `parts` stretches per row. Stretches are of up to 8,192
+// places, shorter where that leaves fewer than two blocks an SM. shifted: a row may need
+// up to 7 places more than it has values.
 struct RowPlan {
   int lanes = 0;  // 0: blocks
   int warps = 1, parts = 1, part_len = 0;
 };
-// Stretches: as few as 8,192 values allow, more where that leaves fewer than two
-// blocks an SM, but none below 1,024 values (a warp's).
-// Mode::kShifted needs up to 7 places more.
-inline RowPlan row_plan(int64_t rows, int64_t codes, bool shifted) {
+inline RowPlan row_plan(int64_t rows, int64_t codes, bool shifted, int vec) {
   RowPlan p;
-  const int64_t room = shifted ? 7 : 0;
-  if (codes + room <= kGroupMaxCodes) {
+  const int64_t places = codes + (shifted ? 7 : 0);
+  if (places <= kGroupMaxCodes) {
     p.lanes = 2;
-    while ((int64_t)p.lanes * kRowElems < codes + room) p.lanes *= 2;
+    while ((int64_t)p.lanes * kRowElems < places) p.lanes *= 2;
     return p;
   }
-  constexpr int64_t kFill = 2 * 148;
-  const int64_t most = kBlockMaxCodes - (shifted ? 8 : 0);
-  int64_t parts = (codes + most - 1) / most;
-  if (rows * parts < kFill) parts = std::max(parts, std::min((codes + 1023) / 1024, (kFill + rows - 1) / rows));
-  const int64_t len = ((codes + parts - 1) / parts + 7) / 8 * 8;  // 16-byte boundaries of every type
-  p.part_len = (int)len;
-  p.parts = (int)((codes + len - 1) / len);
-  while (p.warps * 32 * kRowElems < len + room) p.warps *= 2;
+  p.warps = kBlockMaxWarps;
+  while (p.warps > 1 && (p.warps / 2 * 32 * kRowElems >= places ||
+                         rows * ((places + p.warps * 32 * kRowElems - 1) / (p.warps * 32 * kRowElems)) < 2 * 148))
+    p.warps /= 2;
+  const int64_t most = p.warps * 32 * kRowElems, unit = p.warps * 32 * vec;
+  const int64_t parts = (places + most - 1) / most;
+  p.part_len = (int)(((places + parts - 1) / parts + unit - 1) / unit * unit);
+  p.parts = (int)((places + p.part_len - 1) / p.part_len);
   return p;
 }
 
@@ -434,7 +452,7 @@ inline void with_row_pairs(int32_t dtype, const void* in, int64_t in_stride, con
 inline int check_rows(int32_t dtype, int64_t rows, int64_t codes, int64_t stride, int32_t code_bytes) {
   if (!dtype_ok(dtype)) return GSB_ERR_UNSUPPORTED;
   if (rows < 0 || codes <= 0 || stride < 0 || (code_bytes != 4 && code_bytes != 8)) return GSB_ERR_INVALID_ARGUMENT;
-  if (codes >= (int64_t(1) << 31) - kBlockMaxCodes || rows >= (int64_t(1) << 31)) return GSB_ERR_CAPACITY;
+  if (codes >= (int64_t(1) << 31) - 65536 || rows >= (int64_t(1) << 31)) return GSB_ERR_CAPACITY;
   return GSB_OK;
 }
 

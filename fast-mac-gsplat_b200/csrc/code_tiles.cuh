@@ -164,8 +164,8 @@ struct Range<__half> : PairRange<__half2> {
 
 // Counts of the values of the pieces v0 .. v0 + kTileGroup - 1; 0 where the part has none.
 template <typename T, int L>
-__device__ __forceinline__ void group_counts(const Counts& counts, const Slice<T, L>& at, int v0,
-                                             float (&n)[kTileGroup][wide_of<T>()]) {
+__device__ __forceinline__ void group_counts(const Counts& counts, const Slice<T, L>& at, const Counts::Offsets& off,
+                                             int v0, float (&n)[kTileGroup][wide_of<T>()]) {
   constexpr int VEC = wide_of<T>();
   if (at.shift == 0 && v0 + kTileGroup <= at.w1) {
     const float4* p = reinterpret_cast<const float4*>(counts.by_code + at.at(v0));
@@ -177,11 +177,10 @@ __device__ __forceinline__ void group_counts(const Counts& counts, const Slice<T
         n[v][i] = q.x, n[v][i + 1] = q.y, n[v][i + 2] = q.z, n[v][i + 3] = q.w;
       }
   } else if (VEC == 8 && v0 >= at.w0 && v0 + kTileGroup <= at.w1) {
-    // Codes of one residue modulo 8 lie side by side, as the lanes' pieces of 8 do.
-    const float* p = counts.by_eight + ((at.at(v0) + at.shift) >> 3);
+    const int q = (at.at(v0) + at.shift) >> 3;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const float* pi = p + (((i - at.shift) & 7) * counts.eights - (i < at.shift ? 1 : 0));
+      const float* pi = counts.by_eight + (q + off.of[i % 8]);
 #pragma unroll
       for (int v = 0; v < kTileGroup; ++v) n[v][i] = pi[v * L];
     }
@@ -209,9 +208,10 @@ __device__ __forceinline__ void piece_sums(const LaneBuf& buf, const Slice<T, L>
   constexpr int VEC = wide_of<T>();
   const F2 l2 = f2(kLog2e), neg_M = f2(base.neg_M), neg_n = f2(-r.n);
   F2 s2 = f2(0.0f), w2 = f2(0.0f);
+  const Counts::Offsets off(counts, at.shift);
   for (int v0 = 0; v0 < at.n; v0 += kTileGroup) {
     float n[kTileGroup][VEC];
-    if constexpr (kCounts) group_counts(counts, at, v0, n);
+    if constexpr (kCounts) group_counts(counts, at, off, v0, n);
 #pragma unroll
     for (int v = 0; v < kTileGroup; ++v) {
       float f[VEC];
@@ -317,9 +317,10 @@ __device__ __forceinline__ RowStat lane_sums(const LaneBuf& buf, const Slice<T, 
   r.n = kCounts && some ? counts.by_code[r.a] : 0.0f;
   if (__any_sync(kFullMask, base.far)) {
     r.s = r.w = 0.0f;
+    const Counts::Offsets off(counts, at.shift);
     for (int v0 = 0; v0 < at.n; v0 += kTileGroup) {
       float n[kTileGroup][VEC];
-      if constexpr (kCounts) group_counts(counts, at, v0, n);
+      if constexpr (kCounts) group_counts(counts, at, off, v0, n);
 #pragma unroll
       for (int v = 0; v < kTileGroup; ++v) {
         float f[VEC];

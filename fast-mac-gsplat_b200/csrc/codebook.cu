@@ -57,38 +57,40 @@ __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&v)[V]
 constexpr int kLookupItems = 4;
 constexpr int kLookupPieces = 256 * kLookupItems;  // a block's
 constexpr int kLookupSlots = 2048;                 // that are staged, at most
-template <typename T, typename O, int V, bool kStage>
+template <typename T, typename O, int V, bool kStage, bool kWeights>
 __global__ void __launch_bounds__(256)
-    k_lookup(int64_t pieces, int bag, int64_t C, int nvec, FastDiv div_nvec,
-             const T* __restrict__ table, int64_t stride, Codes codes, const float* __restrict__ weights, float scale,
-             O* __restrict__ out, uint32_t* status) {
+    k_lookup(int64_t pieces, int bag, int64_t C, int nvec, FastDiv div_nvec, const T* __restrict__ table,
+             int64_t stride, Codes codes, const float* __restrict__ weights, float scale, O* __restrict__ out,
+             uint32_t* status) {
   pdl_wait();
   pdl_trigger();
-  __shared__ int2 s_slot[kStage ? kLookupSlots : 1];  // code (-1: none), weight
+  __shared__ int s_at[kStage ? kLookupSlots : 1];  // the row's first value (-1: no row)
+  __shared__ float s_weight[kStage && kWeights ? kLookupSlots : 1];
   const int64_t tile = (int64_t)blockIdx.x * kLookupPieces;
   const int64_t row0 = tile / nvec;
   const int off0 = (int)(tile - row0 * nvec);
-  auto slot = [&](int64_t i) {
-    int64_t c = codes.at(i);
-    if (c >= C) {
-      bad_code(status, kSiteCode);
-      c = -1;
-    }
-    return make_int2(c < 0 ? -1 : (int)c, __float_as_int(weights ? weights[i] : 1.0f));
+  auto row_at = [&](int64_t i) {
+    const int64_t c = codes.at(i);
+    if (c >= C) bad_code(status, kSiteCode);
+    return c < 0 || c >= C ? (int64_t)-1 : c * stride;
   };
+  const int count = (int)min((int64_t)kLookupPieces, pieces - tile);
   if (kStage) {
-    const int64_t last = min(tile + kLookupPieces, pieces) - 1;
-    const int n = (int)(last / nvec - row0 + 1) * bag;
-    for (int i = threadIdx.x; i < n; i += 256) s_slot[i] = slot(row0 * bag + i);
+    const int n = (fast_div(off0 + count - 1, div_nvec) + 1) * bag;
+    for (int i = threadIdx.x; i < n; i += 256) {
+      s_at[i] = (int)row_at(row0 * bag + i);
+      if (kWeights) s_weight[i] = weights[row0 * bag + i];
+    }
     __syncthreads();
   }
   float acc[kLookupItems][V];
   int r[kLookupItems], d[kLookupItems];
 #pragma unroll
   for (int k = 0; k < kLookupItems; ++k) {
-    const int local = min(off0 + k * 256 + (int)threadIdx.x, off0 + (int)min((int64_t)kLookupPieces, pieces - tile) - 1);
+    const int local = off0 + min(k * 256 + (int)threadIdx.x, count - 1);
     r[k] = fast_div(local, div_nvec);
     d[k] = (local - r[k] * nvec) * V;
+    r[k] *= bag;
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[k][i] = 0.0f;
   }
@@ -97,24 +99,35 @@ __global__ void __launch_bounds__(256)
     float w[kLookupItems];
 #pragma unroll
     for (int k = 0; k < kLookupItems; ++k) {
-      const int2 s = kStage ? s_slot[r[k] * bag + j] : slot((row0 + r[k]) * bag + j);
-      w[k] = __int_as_float(s.y);
 #pragma unroll
       for (int i = 0; i < V; ++i) t[k].v[i] = 0.0f;
-      if (s.x >= 0) t[k].load(table + s.x * stride + d[k]);
-      else w[k] = 0.0f;  // an empty slot adds nothing, whatever its weight is
+      w[k] = 0.0f;  // an empty slot adds nothing, whatever its weight is
+      if constexpr (kStage) {
+        const int at = s_at[r[k] + j];
+        if (at >= 0) {
+          t[k].load(table + (at + d[k]));
+          w[k] = kWeights ? s_weight[r[k] + j] : 1.0f;
+        }
+      } else {
+        const int64_t slot = row0 * bag + r[k] + j, at = row_at(slot);
+        if (at >= 0) {
+          t[k].load(table + (at + d[k]));
+          w[k] = kWeights ? weights[slot] : 1.0f;
+        }
+      }
     }
 #pragma unroll
     for (int k = 0; k < kLookupItems; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) acc[k][i] = fmaf(w[k], t[k].v[i], acc[k][i]);
+      for (int i = 0; i < V; ++i) acc[k][i] = kWeights ? fmaf(w[k], t[k].v[i], acc[k][i]) : acc[k][i] + t[k].v[i];
   }
+  O* to = out + tile * V;
 #pragma unroll
   for (int k = 0; k < kLookupItems; ++k) {
-    const int64_t piece = tile + k * 256 + threadIdx.x;
+    const int piece = k * 256 + (int)threadIdx.x;
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[k][i] *= scale;
-    if (piece < pieces) store_vec<V>(out + piece * V, acc[k]);
+    if (piece < count) store_vec<V>(to + piece * V, acc[k]);
   }
 }
 
@@ -553,9 +566,17 @@ extern "C" int gsb_codebook_forward(int32_t table_dtype, int32_t out_dtype, int6
   with_dtypes(table_dtype, out_dtype, [&](auto t, auto o) {
       using T = decltype(t);
       using O = decltype(o);
-      const bool stage = (int64_t)(kLookupPieces / (dim / V) + 2) * bag <= kLookupSlots;
-      auto kernel = V == 4 ? (stage ? k_lookup<T, O, 4, true> : k_lookup<T, O, 4, false>)
-                           : (stage ? k_lookup<T, O, 1, true> : k_lookup<T, O, 1, false>);
+      const bool stage = (int64_t)(kLookupPieces / (dim / V) + 2) * bag <= kLookupSlots &&
+                         codebook_rows * std::max<int64_t>(table_stride, dim) < (int64_t(1) << 31);
+      auto pick = [&](auto v, auto w) {
+        constexpr int W = decltype(v)::value;
+        constexpr bool kWeights = decltype(w)::value;
+        return stage ? k_lookup<T, O, W, true, kWeights> : k_lookup<T, O, W, false, kWeights>;
+      };
+      using One = std::integral_constant<int, 1>;
+      using Four = std::integral_constant<int, 4>;
+      auto kernel = V == 4 ? (weights ? pick(Four{}, std::true_type{}) : pick(Four{}, std::false_type{}))
+                           : (weights ? pick(One{}, std::true_type{}) : pick(One{}, std::false_type{}));
       launch_pdl(kernel, (unsigned)blocks, 256, 0, static_cast<cudaStream_t>(stream), pieces, bag,
                  codebook_rows, dim / V, make_fast_div((uint32_t)(dim / V)),
                  (const T*)table, table_stride, cd, weights, scale, (O*)out, status);
