@@ -178,7 +178,7 @@ TilePlan balance_plan(int64_t rows, int64_t codes, int size, bool shifted) {
                    kBalanceBlocksShort);
 }
 
-// A warp per row joins its stretches' sums.
+// A warp per row joins its parts' sums.
 __global__ void __launch_bounds__(128)
     k_balance_join(int64_t rows, int64_t C, int bag, int parts, Codes codes, const float4* __restrict__ stat,
                    const uint32_t* __restrict__ stat_a, float4* __restrict__ stats, double* __restrict__ sums) {
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(128)
   const int lane = threadIdx.x % 32;
   double sum = 0.0;
   for (int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 32; row < rows; row += (int64_t)gridDim.x * 4) {
-    // A lane without a stretch adds nothing: -inf at an index behind all.
+    // A lane without a part adds nothing: -inf at an index behind all.
     RowStat r{neg_inf(), 0.0f, 0.0f, 0.0f, 0xffffffffu};
     for (int i = lane; i < parts; i += 32) {
       const float4 v = stat[row * parts + i];
@@ -348,6 +348,8 @@ extern "C" int gsb_code_balance_forward(int32_t dtype, int64_t rows, int64_t cod
   if (rc != GSB_OK) return rc;
   if (bag <= 0) return GSB_ERR_INVALID_ARGUMENT;
   if (rows >= (int64_t(1) << 31) / bag) return GSB_ERR_CAPACITY;
+  if (reinterpret_cast<uintptr_t>(stats) % 16 != 0 || reinterpret_cast<uintptr_t>(state) % 16 != 0)
+    return GSB_ERR_INVALID_ARGUMENT;
   if (!loss || !counts || !state || !status || (rows > 0 && (!logits || !codes))) return GSB_ERR_INVALID_ARGUMENT;
   if (!workspace || workspace_bytes < gsb_code_balance_workspace_size(rows, codebook_rows)) return GSB_ERR_WORKSPACE;
   if (rows == 1) logits_stride = 0;
@@ -415,6 +417,8 @@ extern "C" int gsb_code_balance_backward(int32_t dtype, int64_t rows, int64_t co
   if (rc != GSB_OK) return rc;
   if (rows == 0) return GSB_OK;
   if (!logits || !stats || !state || !g_loss || !g_logits) return GSB_ERR_INVALID_ARGUMENT;
+  if (reinterpret_cast<uintptr_t>(stats) % 16 != 0 || reinterpret_cast<uintptr_t>(state) % 16 != 0)
+    return GSB_ERR_INVALID_ARGUMENT;
   if (rows == 1) logits_stride = codebook_rows;  // as the result's
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   with_row_pairs(dtype, logits, logits_stride, g_logits, codebook_rows, [&](auto t, auto m, auto same) {

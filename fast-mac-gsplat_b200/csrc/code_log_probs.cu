@@ -290,7 +290,9 @@ TilePlan log_probs_plan(int64_t rows, int64_t codes, int size, bool shifted, int
                    kLogProbsBlocksSM);
 }
 
-// One warp per row joins its stretches' sums and picks the largest keys.
+// One warp per row joins its parts' sums and picks the largest of their keys, which it
+// keeps in shared memory where they fit.
+constexpr int kJoinKeys = 512;
 template <typename T>
 __global__ void __launch_bounds__(128)
     k_log_probs_join(int64_t rows, int64_t C, int parts, const T* __restrict__ logits, int64_t stride, Codes codes,
@@ -308,14 +310,21 @@ __global__ void __launch_bounds__(128)
     const float4 v = st[i];
     return RowStat{v.x, v.y, v.z, 0.0f, __float_as_uint(v.w)};
   };
-  // A lane without a stretch adds nothing: -inf at an index behind all.
+  // A lane without a part adds nothing: -inf at an index behind all.
   RowStat r{neg_inf(), 0.0f, 0.0f, 0.0f, 0xffffffffu};
+#pragma unroll 4
   for (int i = lane; i < parts; i += 32) r = join<false>(r, stat_at(i));
   r = join_lanes<false, 32>(r);
   const RowResult q = finish(r);
   if (lane == 0) write_row(o, row, r, q, code, code >= 0, zc);
+  __shared__ uint64_t s_keys[4][kJoinKeys];
   const uint64_t* ks = keys + row * parts * top_k;
   const int n = parts * top_k;
+  if (n <= kJoinKeys) {
+    uint64_t* to = s_keys[threadIdx.x / 32];
+    for (int i = lane; i < n; i += 32) to[i] = ks[i];  // each lane looks at its own alone
+    ks = to;
+  }
   uint64_t limit = ~uint64_t(0);
   for (int j = 0; j < top_k; ++j) {
     uint64_t best = 0;
@@ -374,12 +383,16 @@ struct Special {
   int64_t c;  // -1: none
   float own, others, z;
   template <typename T>
-  __device__ __forceinline__ Special(const LogProbsIn& in, const RowGrad& g, int64_t row, int j,
+  __device__ __forceinline__ Special(const LogProbsIn& in, const RowGrad& g, int64_t row, int64_t C, int j,
                                      const T* __restrict__ p) {
     const int k = in.top_k;
+    c = -1;
+    own = others = z = 0.0f;
+    if (j > k || g.empty) return;
     const int32_t* tc = in.top_codes + row * k;
     const float* gt = in.g_top + row * k;
-    c = j < k ? (int64_t)tc[j] : j == k ? g.code : -1;
+    c = j < k ? (int64_t)tc[j] : g.code;
+    if (c >= C) c = -1;
     own = c == g.code ? g.gl : 0.0f;
     others = c == g.code ? 0.0f : g.gl;
     for (int i = 0; i < k; ++i) {
@@ -387,7 +400,6 @@ struct Special {
       if (i == j) own += gt[i];
       else others += gt[i];
     }
-    if (g.empty) c = -1;
     z = c >= 0 ? to_f32(p[c]) : 0.0f;
   }
   template <typename T>
@@ -463,9 +475,13 @@ __global__ void __launch_bounds__(kGroupThreads, kRowThreadsSM / kGroupThreads)
   }
   __syncwarp();  // the second writing comes after the first
   if (row0 + lane32 >= rows) return;
-  for (int j = 0; j <= in.top_k; ++j) {
-    const Special sp(in, g, own, j, logits + own * stride);
+  auto special = [&](int j) { return Special(in, g, own, C, j, logits + own * stride); };
+  auto write = [&](const Special& sp) {
     if (sp.c >= 0) sp.write(g, g_logits + own * C);
+  };
+  for (int j = 0; j <= in.top_k; j += 3) {  // the loads of three places at once
+    const Special s0 = special(j), s1 = special(j + 1), s2 = special(j + 2);
+    write(s0), write(s1), write(s2);
   }
 }
 
@@ -488,7 +504,7 @@ __global__ void __launch_bounds__(W * 32, kRowThreadsSM / (W * 32))
     if constexpr (SAME) load_row(p + c0, at, z);
     else load_row_single(p + c0, at, z);
     const RowGrad g(in, row, C);
-    const Special sp(in, g, row, threadIdx.x <= in.top_k ? (int)threadIdx.x : in.top_k + 1, p);
+    const Special sp(in, g, row, C, (int)threadIdx.x, p);
     const Base base(g.st.x);
     const float beta = g.beta(), alpha = g.alpha(), beta2 = beta * kLn2;
     row_grad(z, base.far && !g.empty, g.st.x, alpha, beta, base.neg_M, (alpha - beta2 * base.d) * base.undo,
@@ -501,7 +517,7 @@ __global__ void __launch_bounds__(W * 32, kRowThreadsSM / (W * 32))
     __syncthreads();  // the second writing comes after the first
     if (sp.c >= max(c0, 0) && sp.c < c0 + hi) sp.write(g, dz);
     if (W == 1 && in.top_k == 32 && threadIdx.x == 0) {  // one place more than threads
-      const Special more(in, g, row, 32, p);
+      const Special more(in, g, row, C, 32, p);
       if (more.c >= max(c0, 0) && more.c < c0 + hi) more.write(g, dz);
     }
   }
@@ -555,6 +571,7 @@ extern "C" int gsb_code_log_probs_forward(int32_t dtype, int64_t rows, int64_t c
   if (!logits || !entropy || !status || (log_probs != nullptr) != (codes != nullptr) ||
       (top_k > 0 && (!top_log_probs || !top_codes)))
     return GSB_ERR_INVALID_ARGUMENT;
+  if (reinterpret_cast<uintptr_t>(stats) % 16 != 0) return GSB_ERR_INVALID_ARGUMENT;
   const size_t need = gsb_code_log_probs_workspace_size(rows, codebook_rows, top_k);
   if (need > 0 && (!workspace || workspace_bytes < need)) return GSB_ERR_WORKSPACE;
   if (rows == 1) logits_stride = 0;
@@ -594,6 +611,7 @@ extern "C" int gsb_code_log_probs_backward(int32_t dtype, int64_t rows, int64_t 
   const int rc = check_log_probs(dtype, rows, codebook_rows, logits_stride, code_bytes, top_k);
   if (rc != GSB_OK) return rc;
   if (rows == 0) return GSB_OK;
+  if (reinterpret_cast<uintptr_t>(stats) % 16 != 0) return GSB_ERR_INVALID_ARGUMENT;
   if (!logits || !stats || !g_logits || (g_log_probs && !codes) || (g_top_log_probs && top_k > 0 && !top_codes))
     return GSB_ERR_INVALID_ARGUMENT;
   if (rows == 1) logits_stride = codebook_rows;  // as the result's

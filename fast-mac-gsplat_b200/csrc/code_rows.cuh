@@ -1,24 +1,22 @@
 // What the row-wise operators on assignment logits z [rows, C] share
-// (code_log_probs.cu, code_balance.cu): reading a stretch of a row into
-// registers, and its softmax sums.
+// (code_log_probs.cu, code_balance.cu): the rule of their softmax sums, the order of
+// alternatives, and the backward's way of reading and writing rows (the forward's is
+// in code_tiles.cuh).
 //
-// Sums over a row are taken over e_c = exp(z_c - m), m = max z. The values equal
-// to m contribute exactly 1 each and are counted, not added:
-//   s' = sum_{z_c < m} e_c + (number of z_c = m) - 1,     p_c = e_c / (1 + s')
+// Sums over a row are taken over e_c = exp(z_c - m), m = max z. The value at a, the
+// first c with z_c = m, contributes exactly 1 and is left out:
+//   s' = sum_{c != a} e_c,     p_c = e_c / (1 + s')
 //   log p_c = (z_c - m) - log1p(s')
-//   t  = sum e_c (z_c - m),  mu = t / (1 + s'),  H = log1p(s') - mu
-//   u  = sum e_c (n_c - n_a), a the first c with z_c = m:  sum p_c n_c = n_a + u / (1 + s')
+//   t  = sum_{c != a} e_c (z_c - m),  mu = t / (1 + s'),  H = log1p(s') - mu
+//   u  = sum_{c != a} e_c (n_c - n_a),     sum_c p_c n_c = n_a + u / (1 + s')
 // so that log p, 1 - p, H and n_c - sum p n keep their relative accuracy where
-// one probability is close to 1 (s' far below 1). All sums are fp32.
+// one probability is close to 1 (s' far below 1). All sums are fp32. Sums of two
+// parts of a row meet by the same rule (join).
 //
-// A row is read once. kRowElems values a lane stay in registers between the
-// maximum and the sums (a second pass over registers costs less than rescaling
-// running sums at every new maximum). Lanes that share a row:
-//   - 2 to 16 for rows of up to 512 values (several rows a warp),
-//   - 1 to 8 warps for rows, or stretches of rows, of up to 8,192 values. Each
-//     warp takes its own maximum and sums; only their results meet.
-// Stretches of a longer row, or of a few rows that would leave the GPU idle, are
-// joined by a second kernel with the same rule (join).
+// The backward is elementwise: kRowElems values a lane in registers, 2 to 16 lanes a
+// row for rows of up to 512 values and 1 to 8 warps for stretches of longer ones; 64
+// registers a thread, which keeps enough loads under way (with 80 it took 4 to 10 %
+// longer).
 #pragma once
 
 #include <algorithm>

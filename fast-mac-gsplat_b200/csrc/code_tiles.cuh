@@ -176,13 +176,13 @@ __device__ __forceinline__ void group_counts(const Counts& counts, const Slice<T
         const float4 q = p[(v * L * VEC + i) / 4];
         n[v][i] = q.x, n[v][i + 1] = q.y, n[v][i + 2] = q.z, n[v][i + 3] = q.w;
       }
-  } else if (VEC == 8 && v0 >= at.w0 && v0 + kTileGroup <= at.w1) {
-    const int q = (at.at(v0) + at.shift) >> 3;
+  } else if (v0 >= at.w0 && v0 + kTileGroup <= at.w1) {
+    const int c = at.at(v0);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const float* pi = counts.by_eight + (q + off.of[i % 8]);
+      const float* p = VEC == 8 ? counts.by_eight + (((c + at.shift) >> 3) + off.of[i % 8]) : counts.by_code + c + i;
 #pragma unroll
-      for (int v = 0; v < kTileGroup; ++v) n[v][i] = pi[v * L];
+      for (int v = 0; v < kTileGroup; ++v) n[v][i] = p[VEC == 8 ? v * L : v * L * VEC];
     }
   } else {
     for (int v = 0; v < kTileGroup; ++v) {
@@ -292,11 +292,12 @@ __device__ __forceinline__ void find_value(const LaneBuf& buf, int v0, float m, 
   *rest = other;
 }
 
-// The softmax sums of one lane's values of a slice, without its largest (its first largest, which leaves `buf` too). The index in the
-// result is the part's. second: the largest of the others (NaN: none).
+// The softmax sums of one lane's values of a slice, without its largest (its first
+// largest, which leaves `buf` too). The index in the result is the part's. second: the
+// largest of the others (NaN: none).
 template <bool kCounts, typename T, int L, typename GroupTop, typename Done>
-__device__ __forceinline__ RowStat lane_sums(const LaneBuf& buf, const Slice<T, L>& at, const Counts& counts, float& second,
-                                             GroupTop&& group_top, Done&& done) {
+__device__ __forceinline__ RowStat lane_sums(const LaneBuf& buf, const Slice<T, L>& at, const Counts& counts,
+                                             float& second, GroupTop&& group_top, Done&& done) {
   constexpr int VEC = wide_of<T>();
   if (at.ragged()) fill_ragged(buf, at, quiet_nan());
   const LaneTop top = lane_top(buf, at, group_top);
@@ -379,7 +380,7 @@ inline TilePlan tile_plan(int64_t rows, int64_t codes, int size, bool shifted, i
       return p;
     }
   }
-  const int64_t slice = 32 * kTilePieces * vec, most = most_slices * slice - 8;
+  const int64_t slice = 32 * kTilePieces * vec, most = most_slices * slice - (shifted ? 8 : 0);
   const int64_t least_parts = (codes + most - 1) / most;
   const int64_t most_parts = std::max(least_parts, std::min<int64_t>((codes + slice / 4 - 1) / (slice / 4), 1024));
   int64_t best_cost = INT64_MAX, best = least_parts;
@@ -405,6 +406,7 @@ inline void with_tile_lanes(int lanes, Fn&& fn) {
 inline bool rows_shifted(int size, const void* p, int64_t stride) {
   return reinterpret_cast<uintptr_t>(p) % 16 != 0 || stride * size % 16 != 0;
 }
+
 // The rows of a call, and where a warp is in them.
 template <typename T>
 struct TileRows {

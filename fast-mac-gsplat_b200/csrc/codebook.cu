@@ -225,7 +225,9 @@ __global__ void __launch_bounds__(1024)
 constexpr int kRunEntries = 16;
 constexpr int kRunBlockEntries = 2048;  // at most, per block
 template <int GL>
-constexpr int run_entries() { return kRunBlockEntries / (256 / GL) < kRunEntries ? kRunBlockEntries / (256 / GL) : kRunEntries; }
+constexpr int run_entries() {
+  return kRunBlockEntries / (256 / GL) < kRunEntries ? kRunBlockEntries / (256 / GL) : kRunEntries;
+}
 template <int GL>
 constexpr int run_block_entries() { return run_entries<GL>() * (256 / GL); }
 
@@ -345,7 +347,8 @@ __global__ void __launch_bounds__(256, WGRAD ? 1 : 4)
   if (s >= e) return;
   // The runs that cross stretches: the group a run starts in takes its tail and
   // the heads after it; group 0 also takes a run from before the block.
-  auto chain = [&](int from) {  // adds the heads of stretches from, from + 1, ... ; true if the run goes on behind the block
+  // Adds the heads of stretches from, from + 1, ...; true if the run goes on behind the block.
+  auto chain = [&](int from) {
     for (int j = from; j < NG; ++j) {
       const float* h = s_part[0][j];
 #pragma unroll
@@ -464,8 +467,9 @@ __global__ void __launch_bounds__(256)
   if (lane == 0) g_weights[i] = acc * scale;
 }
 
-// How the columns of a row are dealt out: V values a piece, GL lanes a row, R = 2
-// or 3 pieces a lane, whichever leaves fewer lanes idle; more columns take more tiles.
+// How the columns of a row are dealt out: V values a piece, GL lanes a row, R pieces a
+// lane (2 or 3 of four values, 2 or 4 single ones), whichever leaves fewer lanes idle,
+// of equals the larger; more columns take more tiles.
 struct RunShape {
   int V, GL, R;
   int block_entries() const {
@@ -476,9 +480,10 @@ struct RunShape {
 };
 RunShape run_shape(int dim, int V) {
   const int nvec = (dim + V - 1) / V;
-  RunShape best{V, 32, 3};
+  const int most = V == 4 ? 3 : 4;
+  RunShape best{V, 32, most};
   int waste = 1 << 30;
-  for (int R = 3; R >= 2; --R) {
+  for (int R : {most, 2}) {
     int GL = 1;
     while (GL < 32 && GL * R < nvec) GL *= 2;
     if (GL * R < nvec) continue;
@@ -516,21 +521,27 @@ void with_dtypes(int32_t table_dtype, int32_t out_dtype, Fn&& fn) {
   });
 }
 
-// Calls fn(integral constants GL, R).
+// Calls fn(integral constants V, GL, R).
 template <typename Fn>
 void with_shape(const RunShape& s, Fn&& fn) {
-  auto lanes = [&](auto r) {
+  auto lanes = [&](auto v, auto r) {
     switch (s.GL) {
-      case 1: fn(std::integral_constant<int, 1>{}, r); break;
-      case 2: fn(std::integral_constant<int, 2>{}, r); break;
-      case 4: fn(std::integral_constant<int, 4>{}, r); break;
-      case 8: fn(std::integral_constant<int, 8>{}, r); break;
-      case 16: fn(std::integral_constant<int, 16>{}, r); break;
-      default: fn(std::integral_constant<int, 32>{}, r); break;
+      case 1: fn(v, std::integral_constant<int, 1>{}, r); break;
+      case 2: fn(v, std::integral_constant<int, 2>{}, r); break;
+      case 4: fn(v, std::integral_constant<int, 4>{}, r); break;
+      case 8: fn(v, std::integral_constant<int, 8>{}, r); break;
+      case 16: fn(v, std::integral_constant<int, 16>{}, r); break;
+      default: fn(v, std::integral_constant<int, 32>{}, r); break;
     }
   };
-  if (s.R == 2) lanes(std::integral_constant<int, 2>{});
-  else lanes(std::integral_constant<int, 3>{});
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  using Three = std::integral_constant<int, 3>;
+  using Four = std::integral_constant<int, 4>;
+  if (s.V == 4 && s.R == 2) lanes(Four{}, Two{});
+  else if (s.V == 4) lanes(Four{}, Three{});
+  else if (s.R == 2) lanes(One{}, Two{});
+  else lanes(One{}, Four{});
 }
 
 // Sizes common to both directions; the blocks of a launch have to fit the grid.
@@ -539,7 +550,7 @@ int check_sizes(int32_t table_dtype, int32_t out_dtype, int64_t rows, int32_t ba
   if (!dtype_ok(table_dtype) || (out_dtype != table_dtype && out_dtype != GSB_DTYPE_F32)) return GSB_ERR_UNSUPPORTED;
   if (rows < 0 || bag <= 0 || codebook_rows <= 0 || dim <= 0 || stride < 0 || (code_bytes != 4 && code_bytes != 8))
     return GSB_ERR_INVALID_ARGUMENT;
-  // Column tiles of the gradient are at least 96 wide and fit the grid's 65,535.
+  // Column tiles of the gradient are at least 64 wide and fit the grid's 65,535.
   if (codebook_rows >= (int64_t(1) << 31) - 1 || rows > kSortMaxN / bag || dim > (1 << 20)) return GSB_ERR_CAPACITY;
   return GSB_OK;
 }
@@ -605,11 +616,12 @@ extern "C" int gsb_codebook_backward(int32_t table_dtype, int32_t out_dtype, int
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t slots = rows * bag;
   if (slots == 0) {
-    if (g_table && cudaMemsetAsync(g_table, 0, (size_t)codebook_rows * dim * dtype_bytes(table_dtype), s) != cudaSuccess)
-      return GSB_ERR_CUDA;
+    const size_t bytes = (size_t)codebook_rows * dim * dtype_bytes(table_dtype);
+    if (g_table && cudaMemsetAsync(g_table, 0, bytes, s) != cudaSuccess) return GSB_ERR_CUDA;
     return GSB_OK;
   }
-  if (!codes || !grad_out || !status || (g_weights && !table)) return GSB_ERR_INVALID_ARGUMENT;
+  if (!codes || !grad_out || !status || (g_weights && !table) || !aligned_to(g_table, 4))
+    return GSB_ERR_INVALID_ARGUMENT;
   const Codes cd{codes, code_bytes == 8};
   cudaError_t e = cudaSuccess;
   if (g_table) {
@@ -644,10 +656,9 @@ extern "C" int gsb_codebook_backward(int32_t table_dtype, int32_t out_dtype, int
     with_dtypes(table_dtype, out_dtype, [&](auto t, auto o) {
         using T = decltype(t);
         using O = decltype(o);
-        with_shape(shape, [&](auto gl, auto r) {
-          constexpr int GL = decltype(gl)::value, R = decltype(r)::value;
-          auto kernel = vec ? (fused ? k_run_sums<T, O, 4, GL, R, true> : k_run_sums<T, O, 4, GL, R, false>)
-                            : (fused ? k_run_sums<T, O, 1, GL, R, true> : k_run_sums<T, O, 1, GL, R, false>);
+        with_shape(shape, [&](auto v, auto gl, auto r) {
+          constexpr int W = decltype(v)::value, GL = decltype(gl)::value, R = decltype(r)::value;
+          auto kernel = fused ? k_run_sums<T, O, W, GL, R, true> : k_run_sums<T, O, W, GL, R, false>;
           launch_pdl(kernel, grid, 256, 0, s, (int)slots, bag, make_fast_div((uint32_t)bag), (int)codebook_rows, dim,
                      (const uint32_t*)b.keys_s, (const uint32_t*)b.vals_s, weights, scale, (const O*)grad_out,
                      (const T*)table, table_stride, (T*)g_table, g_weights, b.parts);

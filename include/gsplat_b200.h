@@ -278,7 +278,8 @@ int gsb_codebook_forward(int32_t table_dtype, int32_t out_dtype, int64_t rows, i
                          const void* codes, int32_t code_bytes, const float* weights, float scale, void* out,
                          uint32_t* status, void* stream);
 /* Its gradients: g_table [codebook_rows, dim] of table_dtype (every row written,
- * zeros where a code is not used) and g_weights [rows, bag]; either may be NULL.
+ * zeros where a code is not used; 4-byte aligned) and g_weights [rows, bag]; either
+ * may be NULL.
  * grad_out [rows, dim] of out_dtype. The codes are sorted (rows * bag < 2^30);
  * the workspace may be NULL without g_table. */
 size_t gsb_codebook_backward_workspace_size(int64_t rows, int32_t bag, int64_t codebook_rows, int32_t dim);
@@ -293,7 +294,7 @@ int gsb_codebook_backward(int32_t table_dtype, int32_t out_dtype, int64_t rows, 
  * the top_k (0 .. GSB_CODE_MAX_TOP) largest log probabilities with their codes,
  * ties to the lower code. A logit of -inf has probability 0; a row of nothing
  * else has log probabilities -inf, entropy 0 and gradient 0. stats [rows, 4]
- * (optional) is what the backward reads. The workspace may be NULL where its
+ * (optional, on a 16-byte boundary) is what the backward reads. The workspace may be NULL where its
  * size is 0. */
 size_t gsb_code_log_probs_workspace_size(int64_t rows, int64_t codebook_rows, int32_t top_k);
 int gsb_code_log_probs_forward(int32_t dtype, int64_t rows, int64_t codebook_rows, const void* logits,
@@ -313,7 +314,7 @@ int gsb_code_log_probs_backward(int32_t dtype, int64_t rows, int64_t codebook_ro
  *   loss = codebook_rows * sum_c f_c P_c      (1 for even use; 0 without any code)
  * and counts [codebook_rows] how often each code occurs. The gradient goes to the
  * logits through P; counts are constants. stats [rows, 4] (optional) and state,
- * gsb_code_balance_state_floats of them on a 16-byte boundary, are what the
+ * gsb_code_balance_state_floats of them, both on 16-byte boundaries, are what the
  * backward reads. rows * bag < 2^31. */
 int64_t gsb_code_balance_state_floats(int64_t codebook_rows);
 size_t gsb_code_balance_workspace_size(int64_t rows, int64_t codebook_rows);

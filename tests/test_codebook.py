@@ -283,6 +283,20 @@ def test_lookup_of_nothing():
 
 
 @pytest.mark.gpu
+def test_lookup_gradient_of_many_slots():
+    """More than 2^22 slots: the sort takes its prefixes another way."""
+    rows, C = (1 << 20) + 77, 3001
+    table, codes, w = _lookup_case(rows, C, (3,), 4, torch.float32, seed=12)
+    w = w.round()  # whole numbers: sums of them are exact below 2^24
+    t = table.detach().requires_grad_(True)
+    g, = torch.autograd.grad(tgb.codebook_lookup(t, codes, w).sum(), t)
+    keep = codes >= 0
+    ref = torch.zeros(C, device=DEV, dtype=torch.float64).index_add_(0, codes[keep].long(), w[keep].double())
+    assert ref.abs().max() < 2**24
+    assert torch.equal(g.double(), ref[:, None].expand(C, 3))
+
+
+@pytest.mark.gpu
 def test_lookup_only_what_is_asked():
     table, codes, w = _lookup_case(100, 9, (5,), 2, torch.float32, seed=30)
     w.requires_grad_(True)
@@ -537,6 +551,44 @@ def test_log_probs_shapes_and_strides(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, C, k", [(101, 7, 3), (70, 61, 2), (40, 129, 9), (37, 255, 4), (9, 1027, 3),
+                                        (5, 5001, 2), (3, 20001, 5)])
+@pytest.mark.parametrize("offset", [1, 3, 6])
+def test_rows_between_16_byte_boundaries(dtype, rows, C, k, offset):
+    """Contiguous rows of odd length from an odd address on: the first row begins inside a
+    16-byte piece whose other values are no part of the tensor."""
+    g = _gen(C + offset)
+    flat = (torch.randn(rows * C + offset + 8, device=DEV, generator=g) * 2.5).to(dtype)
+    flat[:offset], flat[offset + rows * C :] = math.nan, math.nan
+    z = flat[offset : offset + rows * C].view(rows, C)
+    _check_log_probs(z, _codes_for(z, 1), k)
+    codes = torch.randint(-1, C, (rows, 2), device=DEV, generator=g)
+    _check_balance(z, codes, 10.0)
+    assert flat[:offset].isnan().all() and flat[offset + rows * C :].isnan().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("C, k", [(20, 20), (100, 32), (400, 12), (3001, 32)])
+def test_alternatives_around_nan_and_ties(dtype, C, k):
+    """NaN comes after every number, from the lowest code on; equal values by code."""
+    g = _gen(C)
+    z = torch.randint(-2, 3, (33, C), device=DEV, generator=g).to(dtype)  # five values: many ties
+    r = tgb.code_log_probs(z, top_k=k)
+    assert torch.equal(r.top_codes.long(), torch.argsort(z.float(), dim=-1, descending=True, stable=True)[:, :k])
+    z[:, :] = math.nan  # and fewer numbers than alternatives
+    for row in range(33):
+        keep = torch.randperm(C, device=DEV, generator=g)[: min(k // 2, C)]
+        z[row, keep] = torch.randn(keep.numel(), device=DEV, generator=g).to(dtype)
+    r = tgb.code_log_probs(z, top_k=k)
+    low = torch.where(z.isnan(), -INF, z.float())
+    ref = torch.argsort(low, dim=-1, descending=True, stable=True)[:, :k]
+    assert torch.equal(r.top_codes.long(), ref)
+    assert r.log_probs is None and r.entropy.isnan().all() and r.top_log_probs.isnan().all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("C", [12, 500, 9001])
 def test_log_probs_not_finite(C):
     z = torch.zeros(4, C, device=DEV)
@@ -628,6 +680,17 @@ def test_balance_certain_rows_are_relative():
         s = (C - 1) * math.exp(-25.0)
         ref = C * s / (1 + s) ** 2
         assert abs(g[0, 5].item() - ref) <= 4 * (REL_EXP + (C / 32 + 32) * U) * ref
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C", [16, 60, 300, 5000])
+def test_balance_of_many_codes_a_row(C):
+    """More codes a row than lanes that take it."""
+    z = _logits(19, C, torch.bfloat16, seed=C)
+    codes = torch.randint(-1, C, (19, 45), device=DEV, generator=_gen(2))
+    codes[3] = -1
+    codes[4, :44] = -1
+    _check_balance(z, codes, 50.0)
 
 
 @pytest.mark.gpu
