@@ -235,6 +235,7 @@ __device__ __forceinline__ void balance_grad(float k, float4 st, const Deal<T, M
     const float f = k * st.y;
 #pragma unroll
     for (int i = 0; i < kRowElems; i += 4) {
+      if (at.place(i) - at.lane * Deal<T, M>::VEC >= at.hi) continue;  // no lane has any
       float n[4];
       counts.four(at, shift, off, i, n);
 #pragma unroll
@@ -249,7 +250,7 @@ __device__ __forceinline__ void balance_grad(float k, float4 st, const Deal<T, M
              f = f2(k * st.y * base.undo);
 #pragma unroll
     for (int i = 0; i < kRowElems; i += 4) {
-      if (!at.full && at.place(i) - at.lane * Deal<T, M>::VEC >= at.hi) continue;  // no lane has any
+      if (at.place(i) - at.lane * Deal<T, M>::VEC >= at.hi) continue;  // no lane has any
       float n[4];
       counts.four(at, shift, off, i, n);
 #pragma unroll

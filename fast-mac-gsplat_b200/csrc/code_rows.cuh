@@ -228,28 +228,35 @@ struct Counts {
       for (int j = 0; j < 8; ++j) of[j] = ((j - shift) & 7) * (int)counts.eights - (j < shift ? 1 : 0);
     }
   };
-  // Those of a lane's values k .. k + 3, place 0 being code -shift; 0 where it has none.
+  // Those of a lane's values k .. k + 3 (of which some lane has one), place 0 being code
+  // -shift; 0 where the lane has none.
   template <typename T, Mode M>
   __device__ __forceinline__ void four(const Deal<T, M>& at, int shift, const Offsets& off, int k,
                                        float (&n)[4]) const {
     const int c = at.place(k);
     if constexpr (M == Mode::kWide) {
-      const float4 q = c < at.hi ? *reinterpret_cast<const float4*>(by_code + c)
+      const float4 q = at.full || c < at.hi ? *reinterpret_cast<const float4*>(by_code + c)
                                             : make_float4(0.f, 0.f, 0.f, 0.f);
       n[0] = q.x, n[1] = q.y, n[2] = q.z, n[3] = q.w;
     } else if constexpr (M == Mode::kShifted) {
       static_assert(Deal<T, M>::VEC == 8, "values of two bytes");
       const int first = c - k % 8;  // the piece's
-      const bool whole = at.whole(first);
+      const float* p = by_eight + first / 8;
+      if (at.full) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        n[i] = 0.0f;
-        if (whole) n[i] = by_eight[first / 8 + off.of[k % 8 + i]];
-      }
-      if (!at.full && at.ragged(first)) {
+        for (int i = 0; i < 4; ++i) n[i] = p[off.of[k % 8 + i]];
+      } else {
+        const bool whole = at.whole(first);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (at.has(c + i)) n[i] = by_code[c + i - shift];
+        for (int i = 0; i < 4; ++i) {
+          n[i] = 0.0f;
+          if (whole) n[i] = p[off.of[k % 8 + i]];
+        }
+        if (at.ragged(first)) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (at.has(c + i)) n[i] = by_code[c + i - shift];
+        }
       }
     } else {
 #pragma unroll

@@ -185,14 +185,16 @@ __device__ __forceinline__ void group_counts(const Counts& counts, const Slice<T
       for (int v = 0; v < kTileGroup; ++v) n[v][i] = p[VEC == 8 ? v * L : v * L * VEC];
     }
   } else {
+#pragma unroll
     for (int v = 0; v < kTileGroup; ++v) {
       const int c = at.at(v0 + v);
+      if (VEC == 8 && v0 + v >= at.w0 && v0 + v < at.w1) {
+        const float* p = counts.by_eight + ((c + at.shift) >> 3);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float q = at.has(c + i) ? counts.by_code[c + i] : 0.0f;
+        for (int i = 0; i < VEC; ++i) n[v][i] = p[off.of[i % 8]];
+      } else {
 #pragma unroll
-        for (int u = 0; u < kTileGroup; ++u)
-          if (u == v) n[u][i] = q;
+        for (int i = 0; i < VEC; ++i) n[v][i] = at.has(c + i) ? counts.by_code[c + i] : 0.0f;
       }
     }
   }
