@@ -366,7 +366,8 @@ struct RowGrad {
     st = in.stats[row];
     code = in.g_log_probs ? in.codes.at(row) : -1;
     if (code >= C) code = -1;
-    gl = code >= 0 ? in.g_log_probs[row] : 0.0f;
+    gl = in.g_log_probs ? in.g_log_probs[row] : 0.0f;
+    if (code < 0) gl = 0.0f;
     gh = in.g_entropy ? in.g_entropy[row] : 0.0f;
     lead = gl;
     for (int j = 0; j < in.top_k; ++j) lead += in.g_top[row * in.top_k + j];
