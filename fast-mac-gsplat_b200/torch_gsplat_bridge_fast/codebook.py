@@ -16,8 +16,9 @@ rounded once, and every result is the same from call to call. Codes are int32 or
 int64. A negative code is an empty slot; a code of C or more is taken as empty
 and raises RuntimeError from the next call of this module or from
 check_device_errors(). All calls run on the current stream of the tensors'
-device, synchronise nothing and can be captured into a CUDA graph. Gradients of
-gradients are refused. The checks of arguments and the autograd nodes are in the
+device, synchronise nothing and can be captured into a CUDA graph (a captured
+.backward() needs leaves that no live eager graph holds, as in torch everywhere).
+Gradients of gradients are refused. The checks of arguments and the autograd nodes are in the
 native host module; torch.ops.gsplat_b200.codebook_fwd, code_log_probs_fwd and so
 on are the same operators without autograd.
 """
