@@ -241,8 +241,7 @@ __device__ __forceinline__ void balance_grad(float k, float4 st, const Deal<T, M
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float e = ex2_approx((z[i + j] - st.x) * kLog2e);
-        // Takes no part where st.y is 0 (m may be -inf).
-        z[i + j] = st.y == 0.0f ? 0.0f : f * e * ((n[j] - st.w) - st.z);
+        z[i + j] = f * e * ((n[j] - st.w) - st.z);
       }
     }
   } else {
@@ -261,6 +260,10 @@ __device__ __forceinline__ void balance_grad(float k, float4 st, const Deal<T, M
         split(mul2(e, add2(add2(f2(n[j], n[j + 1]), neg_n), neg_dr)), z[i + j], z[i + j + 1]);
       }
     }
+  }
+  if (st.y == 0.0f) {  // takes no part, whatever it holds
+#pragma unroll
+    for (int i = 0; i < kRowElems; ++i) z[i] = 0.0f;
   }
   if (on) store_row(dz, at, z);
 }

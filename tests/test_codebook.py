@@ -669,6 +669,36 @@ def test_balance_masks(C):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("C", [20, 301, 600, 9001])
+def test_balance_rows_without_a_code_may_hold_anything(dtype, C):
+    """They take no part: the loss, and the others' gradient, as if they held zeros, and
+    no gradient of their own."""
+    z = _logits(40, C, dtype, seed=C)
+    codes = torch.randint(0, C, (40, 2), device=DEV, generator=_gen(3))
+    codes[1::4] = -1
+    clean = z.clone()
+    clean[1::4] = 0.0
+    z[1], z[5], z[9], z[13, 2], z[17, 1], z[21] = math.nan, INF, -INF, math.nan, INF, torch.finfo(dtype).max
+    _check_balance(clean, codes, 50.0)
+    got, ref = [], []
+    for x, out in ((z, got), (clean, ref)):
+        x = x.detach().requires_grad_(True)
+        r = tgb.code_balance_loss(x, codes)
+        out += [r.loss.detach(), r.counts, *torch.autograd.grad(r.loss, x, torch.tensor(50.0, device=DEV))]
+    # Rows of a warp may take another way than with zeros beside them: both results are within the bounds of
+    # _check_balance, so within twice those (off is at most the largest count), and each is rounded.
+    d = REL_EXP + (C / 32 + 32) * U
+    n, loss = int(got[1].max()), ref[0].double()
+    _close(got[0], loss, 6 * d * loss + U * loss, torch.float32)
+    assert torch.equal(got[1], ref[1])
+    k = 50.0 * C / int(got[1].sum()) / 30
+    tol = 8 * k * d * torch.softmax(clean.double(), -1) * 2 * n
+    _close(got[2], ref[2].double(), tol + _half_step(dtype) * (ref[2].double().abs() + tol), dtype)
+    assert not got[2][1::4].any() and got[2][0].any()
+
+
+@pytest.mark.gpu
 def test_balance_certain_rows_are_relative():
     """One row, one code: dz at it is k p (1 - p), with 1 - p far below a step of fp32."""
     for C in (24, 3000, 40000):
