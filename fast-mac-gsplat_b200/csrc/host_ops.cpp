@@ -777,11 +777,17 @@ void codebook_done(const Tensor& t) {
   mapped_status().check(t.device().index());
 }
 
+// Sizes that the kernels take as 32-bit numbers.
+void fits_int32(int64_t n, const char* what) {
+  if (n > INT32_MAX) value_error(std::string("gsplat_b200: too many ") + what);
+}
+
 // Rows of contiguous values at any row stride: [C, ...] as [C, dim], [..., C] as [rows, C].
 Tensor table_rows(const Tensor& table) {
   if (table.dim() < 1 || table.size(0) < 1 || table.numel() == 0)
     value_error("gsplat_b200: codebook must be [C,...] with at least one row and value");
   Tensor t = table.dim() == 1 ? table.unsqueeze(1) : table.flatten(1);
+  fits_int32(t.size(1), "values of a codebook row");
   return t.stride(1) == 1 || t.size(1) == 1 ? t : t.contiguous();
 }
 Tensor logit_rows(const Tensor& logits) {
@@ -807,6 +813,7 @@ LookupShape lookup_shape(const Tensor& codebook, const Tensor& codes, const std:
     s.bag = codes.size(-1);
     s.out.pop_back();
   }
+  fits_int32(s.bag, "codes per row");
   s.rows = codes.numel() / s.bag;
   const auto row = codebook.sizes().slice(1);
   s.out.insert(s.out.end(), row.begin(), row.end());
@@ -924,9 +931,11 @@ Tensor op_code_log_probs_bwd(const std::optional<Tensor>& g_log_probs, const std
   const Tensor c = codes.has_value() && codes->defined() ? code_tensor(*codes, logits) : Tensor();
   const Tensor tc = top_codes.contiguous();
   const int64_t rows = z.size(0), top_k = tc.size(-1);
-  auto has = [&](const Tensor& t, int64_t n) { return !t.defined() || (t.is_cuda() && t.numel() == n); };
-  if (!has(gl, rows) || !has(gh, rows) || !has(gt, rows * top_k) || !has(c, rows) || tc.numel() != rows * top_k ||
-      tc.scalar_type() != at::kInt || stats.numel() != rows * 4 || stats.scalar_type() != at::kFloat)
+  auto has = [&](const Tensor& t, int64_t n) {
+    return !t.defined() || (t.device() == z.device() && t.numel() == n);
+  };
+  if (!has(gl, rows) || !has(gh, rows) || !has(gt, rows * top_k) || !has(c, rows) || !has(tc, rows * top_k) ||
+      tc.scalar_type() != at::kInt || !has(stats, rows * 4) || stats.scalar_type() != at::kFloat)
     value_error("gsplat_b200: the gradients do not match the forward's outputs");
   Tensor dz = empty(logits.sizes(), logits.scalar_type(), z.device());
   check(gsb_code_log_probs_backward(dt, rows, z.size(1), z.data_ptr(), z.stride(0),
@@ -952,6 +961,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> op_code_balance_fwd(const Tensor& log
     given.pop_back();
   }
   if (given != lead || bag < 1) value_error("gsplat_b200: codes must have the shape [...] or [...,J] of logits");
+  fits_int32(bag, "codes per row");
   uint32_t* status = codebook_status(z);
   Tensor loss = empty({}, at::kFloat, dev), counts = empty({C}, at::kInt, dev);
   Tensor state = empty({gsb_code_balance_state_floats(C)}, at::kFloat, dev);
@@ -972,6 +982,8 @@ Tensor op_code_balance_bwd(const Tensor& g_loss, const Tensor& logits, const Ten
   const c10::cuda::CUDAGuard guard(logits.device());
   const Tensor z = logit_rows(logits), g = g_loss.to(at::kFloat).contiguous();
   check_same_device(g, logits, "g_loss");
+  check_same_device(stats, logits, "stats");
+  check_same_device(state, logits, "state");
   if (g.numel() != 1 || state.numel() != gsb_code_balance_state_floats(z.size(1)) ||
       state.scalar_type() != at::kFloat || stats.numel() != z.size(0) * 4 || stats.scalar_type() != at::kFloat)
     value_error("gsplat_b200: the gradient does not match the forward's outputs");

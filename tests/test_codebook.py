@@ -922,3 +922,22 @@ def test_learning_codes_through_the_rasterizer():
             down = loss_of(*args)
         # What is left is the third derivative's h^2 / 6, and 2^-24 of the pixels over h.
         assert abs((up - down).item() / (2 * h) - gx.norm().item()) <= 0.05 * gx.norm().item()
+
+@pytest.mark.gpu
+def test_backward_ops_refuse_tensors_of_other_devices():
+    """The registered backward ops check what a caller hands back to them."""
+    ops = torch.ops.gsplat_b200
+    z = _logits(6, 40, torch.float32, seed=1)
+    codes = _codes_for(z, 1).clamp(min=0)
+    _, ent, top, tc, stats = ops.code_log_probs_fwd(z, codes, 3, True)
+    args = [torch.ones(6, device=DEV), torch.ones_like(ent), torch.ones_like(top), z, codes, tc, stats]
+    assert ops.code_log_probs_bwd(*args).shape == z.shape
+    for i in (0, 1, 2, 4, 5, 6):
+        with pytest.raises(ValueError):
+            ops.code_log_probs_bwd(*args[:i], args[i].cpu(), *args[i + 1 :])
+    loss, _, stats, state = ops.code_balance_fwd(z, codes, True)
+    args = [torch.ones_like(loss), z, stats, state]
+    assert ops.code_balance_bwd(*args).shape == z.shape
+    for i in (0, 2, 3):
+        with pytest.raises(ValueError):
+            ops.code_balance_bwd(*args[:i], args[i].cpu(), *args[i + 1 :])
