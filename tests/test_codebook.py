@@ -20,6 +20,7 @@ import torch
 import torch_gsplat_bridge_fast as tgb
 from oracle import torch_ref as TR
 from torch_gsplat_bridge_fast import _native as N
+from torch_gsplat_bridge_fast.rasterize import _ops
 
 U = 2.0**-24
 REL_EXP = 128 * U + 4 * U
@@ -245,6 +246,26 @@ def test_lookup_uneven_use(kind):
     out, (g,) = _check_lookup(table, codes, w, 1.0, torch.float32)
     if kind == "all empty":
         assert not out.any() and not g.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("slots", [1, 31, 32, 33, 1000, 4096, 4097, 8191, 8192, 8193])
+@pytest.mark.parametrize("C", [1, 7, 100_003])
+def test_lookup_gradient_of_few_slots(slots, C):
+    """Small whole numbers, whose sums are exact in any order; codes that tie, empty slots."""
+    g = _gen(slots + C)
+    codes = torch.randint(-1, C, (slots,), device=DEV, generator=g)
+    if C > 1000:
+        codes[::3] = codes[0].item()
+    table = torch.zeros(C, 5, device=DEV, requires_grad=True)
+    up = torch.randint(-8, 9, (slots, 5), device=DEV, generator=g).float()
+    got, = torch.autograd.grad(tgb.codebook_lookup(table, codes), table, up)
+    ref = torch.zeros(C + 1, 5, device=DEV).index_add_(0, torch.where(codes < 0, C, codes), up)[:C]
+    assert torch.equal(got, ref)
+    codes[-1] = C
+    with pytest.raises(RuntimeError, match="out of bounds"):
+        _ops().codebook_bwd(up, table.detach(), codes, None, 1.0, True, False)
+        tgb.check_device_errors()
 
 
 @pytest.mark.gpu
@@ -926,7 +947,7 @@ def test_learning_codes_through_the_rasterizer():
 @pytest.mark.gpu
 def test_backward_ops_refuse_tensors_of_other_devices():
     """The registered backward ops check what a caller hands back to them."""
-    ops = torch.ops.gsplat_b200
+    ops = _ops()
     z = _logits(6, 40, torch.float32, seed=1)
     codes = _codes_for(z, 1).clamp(min=0)
     _, ent, top, tc, stats = ops.code_log_probs_fwd(z, codes, 3, True)
