@@ -42,6 +42,13 @@ __device__ __forceinline__ int64_t given_code(const LogProbsOut& o, const Codes&
   return c < C ? c : -1;
 }
 
+// The largest of a warp's keys.
+__device__ __forceinline__ uint64_t warp_max(uint64_t key) {
+  const uint32_t hi = __reduce_max_sync(kFullMask, (uint32_t)(key >> 32));
+  const uint32_t lo = __reduce_max_sync(kFullMask, (uint32_t)(key >> 32) == hi ? (uint32_t)key : 0u);
+  return (uint64_t)hi << 32 | lo;
+}
+
 // Alternatives of a row that L lanes have in `buf` (a slice holds it all), one by
 // one: every lane has its own largest, taken out of the buffer; the row's largest of
 // those is next, and its lane looks for another.
@@ -198,12 +205,7 @@ __device__ __forceinline__ void list_alternatives(const TilePlace<T, 32>& now, i
         const uint64_t key = order_key(to_f32(now.p[c]), (uint32_t)(now.c0 + c));
         if (key < limit && key > best) best = key;
       }
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) {
-        const uint64_t u = __shfl_xor_sync(kFullMask, best, d);
-        best = u > best ? u : best;
-      }
-      limit = best;
+      limit = best = warp_max(best);
       if (lane == 0) put(j, best);
     }
   }
@@ -291,8 +293,8 @@ TilePlan log_probs_plan(int64_t rows, int64_t codes, int size, bool shifted, int
 }
 
 // One warp per row joins its parts' sums and picks the largest of their keys, which it
-// keeps in shared memory where they fit.
-constexpr int kJoinKeys = 512;
+// keeps in registers where they are few.
+constexpr int kJoinKeys = 16;  // a lane
 template <typename T>
 __global__ void __launch_bounds__(128)
     k_log_probs_join(int64_t rows, int64_t C, int parts, const T* __restrict__ logits, int64_t stride, Codes codes,
@@ -317,27 +319,26 @@ __global__ void __launch_bounds__(128)
   r = join_lanes<false, 32>(r);
   const RowResult q = finish(r);
   if (lane == 0) write_row(o, row, r, q, code, code >= 0, zc);
-  __shared__ uint64_t s_keys[4][kJoinKeys];
   const uint64_t* ks = keys + row * parts * top_k;
   const int n = parts * top_k;
-  if (n <= kJoinKeys) {
-    uint64_t* to = s_keys[threadIdx.x / 32];
-    for (int i = lane; i < n; i += 32) to[i] = ks[i];  // each lane looks at its own alone
-    ks = to;
-  }
+  const bool few = n <= kJoinKeys * 32;
+  uint64_t own[kJoinKeys];
+#pragma unroll
+  for (int i = 0; i < kJoinKeys; ++i) own[i] = few && lane + 32 * i < n ? ks[lane + 32 * i] : 0;
   uint64_t limit = ~uint64_t(0);
   for (int j = 0; j < top_k; ++j) {
     uint64_t best = 0;
-    for (int i = lane; i < n; i += 32) {
-      const uint64_t key = ks[i];
-      if (key < limit && key > best) best = key;
-    }
+    if (few) {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-      const uint64_t u = __shfl_xor_sync(kFullMask, best, d);
-      best = u > best ? u : best;
+      for (int i = 0; i < kJoinKeys; ++i)
+        if (own[i] < limit && own[i] > best) best = own[i];
+    } else {
+      for (int i = lane; i < n; i += 32) {
+        const uint64_t key = ks[i];
+        if (key < limit && key > best) best = key;
+      }
     }
-    limit = best;
+    limit = best = warp_max(best);
     if (lane == 0) {
       o.top_codes[row * top_k + j] = (int32_t)key_index(best);
       o.top_log_probs[row * top_k + j] = q.log_p(key_value(best));
