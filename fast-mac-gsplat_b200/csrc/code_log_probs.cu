@@ -3,6 +3,9 @@
 //
 // A -inf logit has probability 0. In a row of -inf only log p is -inf, H and the
 // gradient are 0. NaN or +inf make a row's results NaN.
+//
+// Forward and backward, of these the forward: 65,536 x 4,096 fp32 with 4 alternatives 555
+// and 230 us (4.7 TB/s), 2,047 x 50,001 fp16 156 and 55, 2^20 x 64 bf16 with 2 161 and 71.
 #include "code_tiles.cuh"
 
 namespace gsb {
@@ -106,9 +109,9 @@ __device__ __forceinline__ void pick_alternatives(const LaneBuf& buf, int lane, 
 // listed and ranked against one another. Many equal values can overrun the list: then
 // the part is searched once for each key.
 constexpr int kTopList = 128;
-// 128 registers a thread: with 80, for 6 blocks, the same kernels took 653 / 169 / 185 us
-// where they take 615 / 164 / 170 (65,536 x 4,096 fp32, 2,047 x 50,001 fp16 and 2^20 x 64
-// bf16, forward and backward).
+// 128 registers a thread: with 80, for 6 blocks, the same kernels took 654 / 170 / 185 us
+// where these took 615 / 164 / 170 (65,536 x 4,096 fp32, 2,047 x 50,001 fp16 and 2^20 x 64
+// bf16, forward and backward, before later steps).
 constexpr int kLogProbsBlocksSM = 4;
 constexpr int kTopSlices = 2;  // of a part with more than one alternative
 constexpr int kTopGroups = kTopSlices * kTilePieces / kTileGroup;
@@ -293,7 +296,8 @@ TilePlan log_probs_plan(int64_t rows, int64_t codes, int size, bool shifted, int
 }
 
 // One warp per row joins its parts' sums and picks the largest of their keys, which it
-// keeps in registers where they are few.
+// keeps in registers where they are few. Latency alone: a call on 1 x 65,536 bf16 with 8
+// alternatives, both kernels, takes 9.3 us (12.0 with the keys in shared memory).
 constexpr int kJoinKeys = 16;  // a lane
 template <typename T>
 __global__ void __launch_bounds__(128)
@@ -437,7 +441,8 @@ __device__ __forceinline__ void row_grad(float (&z)[kRowElems], bool far, float 
 
 // Rows of up to 512 codes, 32 to a warp: what a row costs besides its values is done
 // for 32 rows at once, a lane each; then L lanes a row go through the values of 32 / L
-// rows at a time.
+// rows at a time. 2^20 x 64 bf16: 86 us for 311 MB (134 twice, 43 of what belongs to the
+// rows), 3.6 TB/s; the latency of the loads, with 64 registers a thread.
 template <typename T, Mode M, bool SAME, int L>
 __global__ void __launch_bounds__(kGroupThreads, kRowThreadsSM / kGroupThreads)
     k_log_probs_bwd_group(int64_t rows, int C, const T* __restrict__ logits, int64_t stride, LogProbsIn in,
@@ -488,6 +493,8 @@ __global__ void __launch_bounds__(kGroupThreads, kRowThreadsSM / kGroupThreads)
 }
 
 // Longer rows: W warps a stretch of the result (SAME: the logits' rows lie alike).
+// 16,384 x 4,096 fp32: 92 us, 5.8 TB/s; 2,047 x 50,001 fp16, rows between 16-byte
+// boundaries, 105 us, 3.9 TB/s: half of the instruction slots.
 template <typename T, Mode M, bool SAME, int W>
 __global__ void __launch_bounds__(W * 32, kRowThreadsSM / (W * 32))
     k_log_probs_bwd_block(int64_t items, int64_t C, int parts, int part_len, const T* __restrict__ logits,

