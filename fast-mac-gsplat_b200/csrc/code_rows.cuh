@@ -61,16 +61,6 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 template <typename T>
 constexpr int wide_of() { return 16 / (int)sizeof(T); }
 
-// NaN in every element of a word: a place without a value, which loses against any.
-template <typename T>
-__device__ __forceinline__ uint32_t nan_bits();
-template <>
-__device__ __forceinline__ uint32_t nan_bits<float>() { return 0x7fc00000u; }
-template <>
-__device__ __forceinline__ uint32_t nan_bits<__nv_bfloat16>() { return 0x7fc07fc0u; }
-template <>
-__device__ __forceinline__ uint32_t nan_bits<__half>() { return 0x7e007e00u; }
-
 // How a stretch of a row is dealt out to `lanes` lanes: lane l's value k has the
 // place (k / VEC lanes + l) VEC + k % VEC. VEC is 1, or the values of a 16-byte piece.
 // Where rows begin between 16-byte boundaries (Mode::kShifted) places count from the
@@ -336,16 +326,6 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
   float r;
   asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
-}
-// Largest of a lane's values (NaN loses), by way of its eight runs of four.
-__device__ __forceinline__ float lane_max(const float (&z)[kRowElems], float (&four)[8]) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) four[j] = fmaxf(max3(z[4 * j], z[4 * j + 1], z[4 * j + 2]), z[4 * j + 3]);
-  return max3(max3(four[0], four[1], four[2]), max3(four[3], four[4], four[5]), fmaxf(four[6], four[7]));
-}
-__device__ __forceinline__ float lane_max(const float (&z)[kRowElems]) {
-  float four[8];
-  return lane_max(z, four);
 }
 // Smallest of a lane's values (NaN loses).
 __device__ __forceinline__ float lane_min(const float (&z)[kRowElems]) {
