@@ -179,8 +179,7 @@ __global__ void __launch_bounds__(kTileWarps * 32, L < 32 ? kBalanceBlocksShort 
   }
 }
 TilePlan balance_plan(int64_t rows, int64_t codes, int size, bool shifted) {
-  return tile_plan(std::max<int64_t>(rows, 1), codes, size, shifted, 1 << 20, kBalanceBlocksLong,
-                   kBalanceBlocksShort);
+  return tile_plan(rows, codes, size, shifted, 1 << 20, kBalanceBlocksLong, kBalanceBlocksShort);
 }
 
 // A warp per row joins its parts' sums. Latency alone: 4 to 6 us.

@@ -375,6 +375,7 @@ struct TilePlan {
 inline TilePlan tile_plan(int64_t rows, int64_t codes, int size, bool shifted, int64_t most_slices, int blocks_sm,
                           int blocks_sm_short) {
   TilePlan p;
+  rows = std::max<int64_t>(rows, 1);
   p.blocks_sm = blocks_sm;
   const int64_t resident = 148 * blocks_sm * kTileWarps;
   const int vec = 16 / size;
@@ -390,11 +391,18 @@ inline TilePlan tile_plan(int64_t rows, int64_t codes, int size, bool shifted, i
   const int64_t least_parts = (codes + most - 1) / most;
   const int64_t most_parts = std::max(least_parts, std::min<int64_t>((codes + slice / 4 - 1) / (slice / 4), 1024));
   int64_t best_cost = INT64_MAX, best = least_parts;
-  for (int64_t parts = least_parts; parts <= most_parts; ++parts) {
+  auto consider = [&](int64_t parts) {
     const int64_t rounds = (rows * parts + resident - 1) / resident;
     const int64_t cost = rounds * ((codes + parts - 1) / parts + slice / 4) + (parts > 1 ? slice / 2 : 0);
     if (cost < best_cost) best_cost = cost, best = parts;
-    if (rounds > 8) break;  // even enough from here on
+  };
+  consider(least_parts);
+  // Of the numbers of parts that make as many rounds the largest is best, or a smaller one
+  // with parts as long. More than 16 rounds are even enough.
+  for (int64_t rounds = (rows * least_parts + resident - 1) / resident; rounds <= 16; ++rounds) {
+    const int64_t parts = std::min(most_parts, rounds * resident / rows), len = (codes + parts - 1) / parts;
+    if (parts > least_parts) consider(std::max(least_parts, (codes + len - 1) / len));
+    if (parts == most_parts) break;
   }
   p.part_len = ((codes + best - 1) / best + 7) / 8 * 8;
   p.parts = (int)((codes + p.part_len - 1) / p.part_len);
