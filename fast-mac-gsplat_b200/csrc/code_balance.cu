@@ -5,8 +5,8 @@
 // columns are needed: with the counts at hand each row is one weighted softmax sum
 // (code_rows.cuh), read once. The sums of d over rows are 64-bit, in a fixed order.
 //
-// Forward and backward, of these the pass over the rows: 2^20 x 256 bf16 333 and 139 us
-// (3.9 TB/s; instructions, of which a count a value), 16,384 x 16,383 fp16 463 and 190,
+// Forward and backward, of these the pass over the rows: 2^20 x 256 bf16 335 and 139 us
+// (3.9 TB/s; instructions, of which a count a value), 16,384 x 16,383 fp16 468 and 190,
 // 65,536 x 1,000 fp32 forward alone 64 and 55 (4.8 TB/s).
 #include "code_tiles.cuh"
 
