@@ -418,13 +418,21 @@ struct Special {
   }
 };
 
-// e (alpha + beta x) of a lane's values, in place (far: Base does not hold); 0 at -inf.
+// The factor of y = x log2 e in a row's gradient, b2, up to which the short way of
+// row_grad holds: beside it y, at least kLowestGrad log2 e, makes no product beyond fp32
+// (1e19 x 1.5e18; a masked place has e = 0, and 0 times infinity is NaN). Larger ones come
+// of incoming gradients above 1e19.
+constexpr float kLowestGrad = -1e18f;
+constexpr float kLargestFactor = 1e19f;
+
+// e (alpha + beta x) of a lane's values, in place (far: Base does not hold, or b2 is too
+// large); 0 wherever e is, at -inf and at any value far enough below m.
 __device__ __forceinline__ void row_grad(float (&z)[kRowElems], bool far, float m, float alpha, float beta,
                                          float neg_M, float a2, float b2) {
-  if (__any_sync(kFullMask, far || lane_min(z) < kLowest)) {
+  if (__any_sync(kFullMask, far || lane_min(z) < kLowestGrad)) {
 #pragma unroll
     for (int i = 0; i < kRowElems; ++i) {
-      const float x = max_nan(z[i] - m, -200.0f);  // e is 0, and beta x finite
+      const float x = max_nan(z[i] - m, -128.0f);  // e is 0, and beta x finite up to beta = 2.6e36
       z[i] = ex2_approx(x * kLog2e) * fmaf(beta, x, alpha);
     }
   } else {
@@ -457,7 +465,7 @@ __global__ void __launch_bounds__(kGroupThreads, kRowThreadsSM / kGroupThreads)
   const Base base(g.st.x);
   const float beta = g.beta(), alpha = g.alpha(), beta2 = beta * kLn2;
   const float b2 = beta2 * base.undo, a2 = (alpha - beta2 * base.d) * base.undo;
-  const bool far = base.far && !g.empty;  // an empty row's values are not used
+  const bool far = (base.far || !(fabsf(b2) <= kLargestFactor)) && !g.empty;  // an empty row's values are not used
 #pragma unroll 1
   for (int h = 0; h < L; ++h) {
     const int from = h * (32 / L) + lane32 / L;
@@ -516,8 +524,9 @@ __global__ void __launch_bounds__(W * 32, kRowThreadsSM / (W * 32))
     const Special sp(in, g, row, C, (int)threadIdx.x, p);
     const Base base(g.st.x);
     const float beta = g.beta(), alpha = g.alpha(), beta2 = beta * kLn2;
-    row_grad(z, base.far && !g.empty, g.st.x, alpha, beta, base.neg_M, (alpha - beta2 * base.d) * base.undo,
-             beta2 * base.undo);
+    const float b2 = beta2 * base.undo, a2 = (alpha - beta2 * base.d) * base.undo;
+    const bool far = (base.far || !(fabsf(b2) <= kLargestFactor)) && !g.empty;
+    row_grad(z, far, g.st.x, alpha, beta, base.neg_M, a2, b2);
     if (g.empty) {
 #pragma unroll
       for (int i = 0; i < kRowElems; ++i) z[i] = 0.0f;

@@ -962,3 +962,35 @@ def test_backward_ops_refuse_tensors_of_other_devices():
     for i in (0, 2, 3):
         with pytest.raises(ValueError):
             ops.code_balance_bwd(*args[:i], args[i].cpu(), *args[i + 1 :])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("C", [40, 41, 600, 9001])
+@pytest.mark.parametrize("low", [-1e4, -1e18, -1e30, -1e34, -1e37, -9e37])
+def test_entropy_gradient_at_very_low_logits(dtype, C, low):
+    """Finite values far below the others (masks of a large number): their gradient is 0, the others' what it is
+    without them, whatever the size of the incoming gradient. fp16 has no such values."""
+    z = _logits(7, C, dtype, seed=C)
+    z[0, 1::2] = low
+    z[1, :-1] = low  # one code stands: p = 1, H = 0
+    z[2] = low  # an even row
+    z[3, 2:] = low
+    z[3, :2] = 0.5  # two even codes
+    z[4, :] += 2000.0
+    z[4, C // 2 :] = low
+    z[5, : C // 2] = low
+    z[5, C // 3] = low * 1.5
+    x = z.double()
+    lp = torch.log_softmax(x, -1)
+    p = lp.exp()
+    H = -(p * lp.clamp(min=-1e6)).sum(-1, keepdim=True)
+    t = torch.where(p > 0, lp + H, 0.0)
+    d = REL_EXP + (C / 32 + 32) * U
+    for rows in (slice(0, 7), *(slice(i, i + 1) for i in range(7))):  # rows of a warp may go one way together
+        for gh in (1.0, 10.0, 64.0, 65536.0, 1e9, 1e30):
+            leaf = z[rows].detach().requires_grad_(True)
+            ent = tgb.code_log_probs(leaf).entropy
+            dz, = torch.autograd.grad(ent, leaf, torch.full_like(ent, gh))
+            q, u = p[rows], t[rows]
+            _close(dz, -gh * q * u, 4 * d * gh * q * (u.abs() + 1 + math.log(C)), dtype)
