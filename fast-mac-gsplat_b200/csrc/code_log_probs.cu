@@ -257,13 +257,13 @@ __global__ void __launch_bounds__(kTileWarps * 32, kLogProbsBlocksSM)
       },
       [&](const TilePlace<T, L>& now, const Slice<T, L>& at, const LaneBuf& buf) {
         RowStat r = join_lanes<false, L>(sums);
-        if (r.a == 0xffffffffu) r.a = (uint32_t)now.c0;  // NaN alone
+        const bool nan_alone = r.a == 0xffffffffu;
         if (L < 32 || t.parts == 1) {
           const RowResult q = finish(r);
           if (now.on && lane == 0) {
             write_row(o, now.row, r, q, code, code >= 0, zc);
             if (top_k == 1) {
-              o.top_codes[now.row] = (int32_t)r.a;
+              o.top_codes[now.row] = nan_alone ? 0 : (int32_t)r.a;
               o.top_log_probs[now.row] = q.log_p(r.m);
             }
           }
@@ -279,7 +279,8 @@ __global__ void __launch_bounds__(kTileWarps * 32, kLogProbsBlocksSM)
         } else if constexpr (L == 32) {
           if (lane32 == 0) stat[now.item] = make_float4(r.m, r.s, r.w, __uint_as_float(r.a));
           uint64_t* to = keys + now.item * top_k;
-          if (top_k == 1 && lane32 == 0) to[0] = order_key(r.m, r.a);
+          if (top_k == 1 && lane32 == 0)
+            to[0] = nan_alone ? order_key(quiet_nan(), (uint32_t)now.c0) : order_key(r.m, r.a);
           if (top_k > 1) {
             const int k = min(top_k, now.len);
             list_alternatives(now, lane32, sums, second, k, *tops, [&](int j, uint64_t key) { to[j] = key; });

@@ -994,3 +994,20 @@ def test_entropy_gradient_at_very_low_logits(dtype, C, low):
             dz, = torch.autograd.grad(ent, leaf, torch.full_like(ent, gh))
             q, u = p[rows], t[rows]
             _close(dz, -gh * q * u, 4 * d * gh * q * (u.abs() + 1 + math.log(C)), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, C", [(1, 70001), (2, 30011), (1, 262147), (3, 9001), (2, 40)])
+def test_best_code_behind_nan(dtype, rows, C):
+    """NaN comes after -inf too, where a row is split into parts and some of them hold NaN alone."""
+    first = C // 2 + 3
+    z = torch.full((rows, C), -INF, device=DEV, dtype=dtype)
+    z[:, :first] = math.nan
+    for k in (1, 2):
+        r = tgb.code_log_probs(z, top_k=k)
+        assert r.top_codes.tolist() == [list(range(first, first + k))] * rows and r.top_log_probs.isnan().all()
+    z[-1] = math.nan
+    assert tgb.code_log_probs(z, top_k=1).top_codes[-1].item() == 0
+    z[:, -1] = -3.0
+    assert tgb.code_log_probs(z, top_k=1).top_codes[:, 0].tolist() == [C - 1] * rows
