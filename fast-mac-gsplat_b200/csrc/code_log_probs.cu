@@ -163,17 +163,17 @@ __device__ __forceinline__ void list_alternatives(const TilePlace<T, 32>& now, i
 #pragma unroll
     for (int v = 0; v < kTileGroup; ++v) {
       const int c = at.at(v0 + v);
-      T e[VEC];
+      Piece<T> e;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) e[i] = from_f32<T>(quiet_nan());
-      q[v] = *reinterpret_cast<const uint4*>(e);
+      q[v] = e.bits();
       if (c >= 0 && c + VEC <= at.len) {
         q[v] = *reinterpret_cast<const uint4*>(now.p + c);
       } else if (c < at.len && c + VEC > 0) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
           if (at.has(c + i)) e[i] = now.p[c + i];
-        q[v] = *reinterpret_cast<const uint4*>(e);
+        q[v] = e.bits();
       }
     }
 #pragma unroll

@@ -118,13 +118,13 @@ __device__ __forceinline__ void load_row(const T* __restrict__ p, const Deal<T, 
         if (at.whole(c)) {
           q[v] = *reinterpret_cast<const uint4*>(p + c);
         } else if (M == Mode::kShifted && at.ragged(c)) {
-          T e[VEC];
+          Piece<T> e;
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
             e[i] = from_f32<T>(0.0f);
             if (at.has(c + i)) e[i] = p[c + i];
           }
-          q[v] = *reinterpret_cast<const uint4*>(e);
+          q[v] = e.bits();
         }
       }
     }
@@ -174,10 +174,10 @@ __device__ __forceinline__ void store_row(T* __restrict__ p, const Deal<T, M>& a
     }
   } else {
     auto piece = [&](int v) {
-      T e[VEC];
+      Piece<T> e;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) e[i] = from_f32<T>(d[v * VEC + i]);
-      return *reinterpret_cast<const uint4*>(e);
+      return e.bits();
     };
     if (at.full) {
 #pragma unroll

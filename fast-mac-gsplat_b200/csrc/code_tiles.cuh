@@ -107,13 +107,13 @@ __device__ __forceinline__ void copy_ragged(const LaneBuf& buf, const T* __restr
 template <typename T, int L>
 __device__ __forceinline__ void fill_ragged(const LaneBuf& buf, const Slice<T, L>& at, float value) {
   constexpr int VEC = wide_of<T>();
-  T e[VEC];
+  Piece<T> e;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) e[i] = from_f32<T>(value);
   at.each_ragged([&](int v) {
     const int c = at.at(v);
     if (c >= at.len || c + VEC <= 0) {
-      buf[v] = *reinterpret_cast<const uint4*>(e);
+      buf[v] = e.bits();
     } else if (c < 0 || c + VEC > at.len) {
       for (int i = 0; i < VEC; ++i)
         if (!at.has(c + i)) reinterpret_cast<T*>(&buf[v])[i] = e[0];

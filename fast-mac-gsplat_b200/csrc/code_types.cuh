@@ -22,6 +22,16 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 
+// The values of 16 bytes, on such a boundary wherever they live.
+template <typename T>
+struct Piece {
+  alignas(16) T v[16 / sizeof(T)];
+  __device__ __forceinline__ T& operator[](int i) { return v[i]; }
+  __device__ __forceinline__ uint4 bits() const { return *reinterpret_cast<const uint4*>(v); }
+};
+static_assert(alignof(Piece<float>) == 16 && sizeof(Piece<float>) == 16, "read as one uint4");
+static_assert(alignof(Piece<__half>) == 16 && sizeof(Piece<__half>) == 16, "read as one uint4");
+
 // Codes are int32 or int64 values; a negative one is an empty slot.
 struct Codes {
   const void* p;

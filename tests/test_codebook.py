@@ -13,6 +13,8 @@ no others).
 from __future__ import annotations
 
 import math
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -1011,3 +1013,15 @@ def test_best_code_behind_nan(dtype, rows, C):
     assert tgb.code_log_probs(z, top_k=1).top_codes[-1].item() == 0
     z[:, -1] = -3.0
     assert tgb.code_log_probs(z, top_k=1).top_codes[:, 0].tolist() == [C - 1] * rows
+
+
+# ---- the sources ---------------------------------------------------------------
+def test_local_arrays_read_wide_are_aligned():
+    """A local array of narrow values that is read as one 16-byte (or 8-byte) value lies on such a boundary
+    only if it says so: nothing else promises it once the array is in memory."""
+    csrc = Path(N.__file__).resolve().parents[1] / "csrc"
+    for path in sorted((*csrc.glob("*.cu"), *csrc.glob("*.cuh"))):
+        text = path.read_text()
+        for name in set(re.findall(r"\*reinterpret_cast<(?:const )?(?:uint|int|float)[24]\*>\((\w+)\)", text)):
+            plain = re.findall(rf"^\s*(?!extern|__shared__|.*__align__|.*alignas)[\w:<>]+ {name}\[[^]]*\];", text, re.M)
+            assert not plain, f"{path.name}: {plain}"
