@@ -41,13 +41,16 @@ struct Codes {
   }
 };
 
-// A code of at least n: recorded, and treated as an empty slot. The status
-// block may be mapped host memory, so this is a plain (posted) store: a million
-// bad codes cost no round trips.
-__device__ __forceinline__ void bad_code(uint32_t* status, uint32_t site) {
+// An error of these kernels. The status block may be mapped host memory, so these are
+// plain (posted) stores: a million bad codes cost no round trips.
+__device__ __forceinline__ void put_error(uint32_t* status, uint32_t flag, uint32_t site) {
   if (status == nullptr) return;
   st_volatile_u32(&status[GSB_STATUS_ERROR_SITE], site);
-  st_volatile_u32(&status[GSB_STATUS_ERROR], GSB_DEVERR_BOUNDS);
+  st_volatile_u32(&status[GSB_STATUS_ERROR], flag);
+}
+// A code of at least n: recorded, and treated as an empty slot.
+__device__ __forceinline__ void bad_code(uint32_t* status, uint32_t site) {
+  put_error(status, GSB_DEVERR_BOUNDS, site);
 }
 
 inline bool dtype_ok(int32_t d) { return d == GSB_DTYPE_F32 || d == GSB_DTYPE_BF16 || d == GSB_DTYPE_F16; }

@@ -153,7 +153,7 @@ constexpr int kKeyItems = 8;
 __global__ void __launch_bounds__(256)
     k_code_keys(int64_t n, int64_t C, int passes, Codes codes, uint32_t* __restrict__ keys,
                 uint32_t* __restrict__ vals, uint32_t* __restrict__ digits, uint32_t* __restrict__ zero,
-                int64_t zero_bytes, uint32_t* status) {
+                int64_t zero_bytes, uint32_t* __restrict__ sort_status, uint32_t* status) {
   pdl_wait();
   pdl_trigger();
   __shared__ uint32_t s_digits[4][kRadix];
@@ -171,6 +171,7 @@ __global__ void __launch_bounds__(256)
     }
   }
   zero_words(zero, zero_bytes);
+  if (blockIdx.x == 0 && threadIdx.x < GSB_STATUS_WORDS) sort_status[threadIdx.x] = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < passes * kRadix; i += 256) {
     const uint32_t v = (&s_digits[0][0])[i];
@@ -244,6 +245,10 @@ __global__ void __launch_bounds__(256)
 // takes the row in one tile of columns. 2^20 x 48 fp32 of 8,192 codes: 50 us, 4.8 TB/s
 // read. Four of 27 bf16 for 100,003 rows, with g_w: 30 us; rows of 54 bytes come a value
 // at a time, out of L2.
+//
+// sort_status (NULL: nothing waited): the words of the sort that made the order, its own
+// because it gives up waiting when they hold an error, which the call's may from earlier
+// calls and other streams. An order that was given up is no permutation and not followed.
 constexpr int kRunEntries = 16;
 constexpr int kRunBlockEntries = 2048;  // at most, per block
 template <int GL>
@@ -258,7 +263,8 @@ __global__ void __launch_bounds__(256, WGRAD ? 1 : 4)
     k_run_sums(int n, int bag, FastDiv div_bag, int C, int dim, const uint32_t* __restrict__ keys,
                const uint32_t* __restrict__ vals, const float* __restrict__ weights, float scale,
                const O* __restrict__ g, const T* __restrict__ table, int64_t stride, T* __restrict__ g_table,
-               float* __restrict__ g_weights, float* __restrict__ parts) {
+               float* __restrict__ g_weights, float* __restrict__ parts, const uint32_t* __restrict__ sort_status,
+               uint32_t* status) {
   pdl_wait();
   pdl_trigger();
   constexpr int NG = 256 / GL, E = run_entries<GL>(), L = run_block_entries<GL>(), W = GL * V * R;
@@ -272,10 +278,15 @@ __global__ void __launch_bounds__(256, WGRAD ? 1 : 4)
   const int64_t b0 = (int64_t)blockIdx.x * L;
   const int cnt = (int)min((int64_t)L, n - b0);
   const uint32_t kNone = 0xffffffffu;  // no entry: differs from every key
+  const bool given_up = sort_status != nullptr && sort_status[GSB_STATUS_ERROR] != 0;
   for (int i = tid; i < L + 2; i += 256) {
     const int64_t k = b0 + i - 1;
     s_key[i] = k >= 0 && k < n ? keys[k] : kNone;
     if (i >= 1 && i <= L) s_val[i - 1] = i <= cnt ? vals[k] : 0u;
+  }
+  if (given_up) {
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) put_error(status, GSB_DEVERR_LOOKBACK_TIMEOUT, kSiteSortLookback);
+    return;
   }
   __syncthreads();
   const int col0 = (int)blockIdx.y * W + lane * V;
@@ -521,6 +532,7 @@ RunShape run_shape(int dim, int V) {
 
 struct BackwardScratch {
   uint32_t *keys = nullptr, *vals = nullptr, *keys_s = nullptr, *vals_s = nullptr;
+  uint32_t* sort_status = nullptr;
   float* parts = nullptr;
 };
 BackwardScratch carve(Carver& ws, int64_t slots, int dim) {
@@ -529,6 +541,7 @@ BackwardScratch carve(Carver& ws, int64_t slots, int dim) {
   b.vals = ws.take<uint32_t>((size_t)slots);
   b.keys_s = ws.take<uint32_t>((size_t)slots);
   b.vals_s = ws.take<uint32_t>((size_t)slots);
+  b.sort_status = ws.take<uint32_t>(GSB_STATUS_WORDS);
   const int64_t least = std::min(run_shape(dim, 1).block_entries(), run_shape(dim, 4).block_entries());
   b.parts = ws.take<float>((size_t)((slots + least - 1) / least) * 2 * (size_t)dim);
   return b;
@@ -655,7 +668,8 @@ extern "C" int gsb_codebook_backward(int32_t table_dtype, int32_t out_dtype, int
     const BackwardScratch b = carve(ws, slots, dim);
     const int64_t table_bytes = codebook_rows * dim * dtype_bytes(table_dtype);
     const int zero_blocks = (int)std::min<int64_t>(148 * 8, (table_bytes + (1 << 14) - 1) >> 14);
-    if (slots <= kFewSlots) {
+    const bool few = slots <= kFewSlots;
+    if (few) {
       const int blocks = std::max(zero_blocks, ((int)slots + kRankBlock - 1) / kRankBlock);
       launch_pdl(k_rank_few, blocks, 256, 0, s, (int)slots, codebook_rows, cd, b.keys_s, b.vals_s,
                  (uint32_t*)g_table, table_bytes, status);
@@ -666,9 +680,9 @@ extern "C" int gsb_codebook_backward(int32_t table_dtype, int32_t out_dtype, int
       if (cudaMemsetAsync(zero.ptr, 0, zero.words * sizeof(uint32_t), s) != cudaSuccess) return GSB_ERR_CUDA;
       const int blocks = std::max(zero_blocks, (int)std::min<int64_t>(148 * 8, grid1d(slots, 256 * kKeyItems)));
       launch_pdl(k_code_keys, blocks, 256, 0, s, slots, codebook_rows, sort_passes(0, bits), cd, b.keys, b.vals,
-                 zero.ptr, (uint32_t*)g_table, table_bytes, status);
+                 zero.ptr, (uint32_t*)g_table, table_bytes, b.sort_status, status);
       note_launches(1);
-      e = radix_sort_pairs(ws, b.keys, b.vals, b.keys_s, b.vals_s, slots, 0, bits, status, s, true, zero.ptr);
+      e = radix_sort_pairs(ws, b.keys, b.vals, b.keys_s, b.vals_s, slots, 0, bits, b.sort_status, s, true, zero.ptr);
       if (e != cudaSuccess) return GSB_ERR_CUDA;
     }
     const int so = dtype_bytes(out_dtype), st = dtype_bytes(table_dtype);
@@ -686,7 +700,8 @@ extern "C" int gsb_codebook_backward(int32_t table_dtype, int32_t out_dtype, int
           auto kernel = fused ? k_run_sums<T, O, W, GL, R, true> : k_run_sums<T, O, W, GL, R, false>;
           launch_pdl(kernel, grid, 256, 0, s, (int)slots, bag, make_fast_div((uint32_t)bag), (int)codebook_rows, dim,
                      (const uint32_t*)b.keys_s, (const uint32_t*)b.vals_s, weights, scale, (const O*)grad_out,
-                     (const T*)table, table_stride, (T*)g_table, g_weights, b.parts);
+                     (const T*)table, table_stride, (T*)g_table, g_weights, b.parts,
+                     few ? (const uint32_t*)nullptr : (const uint32_t*)b.sort_status, status);
         });
         if (grid.x > 1)
           launch_pdl(k_run_parts<T>, grid.x - 1, 256, 0, s, (int)slots, (int)codebook_rows, dim, block_entries,

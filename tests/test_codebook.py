@@ -1015,6 +1015,37 @@ def test_best_code_behind_nan(dtype, rows, C):
     assert tgb.code_log_probs(z, top_k=1).top_codes[:, 0].tolist() == [C - 1] * rows
 
 
+@pytest.mark.gpu
+def test_lookup_gradient_beside_errors_of_other_calls():
+    """Status words that hold an earlier call's error: the sort's waits must not take it for their own. Two
+    streams at once, so that blocks wait for others; whole numbers, whose sums are exact."""
+    L = N.load()
+    n, C = (1 << 21) + 5, 70_003
+    g = _gen(9)
+    codes = torch.randint(-1, C, (n,), device=DEV, generator=g, dtype=torch.int32)
+    up = torch.randint(-8, 9, (n,), device=DEV, generator=g).float()
+    ref = torch.zeros(C + 1, device=DEV).index_add_(0, torch.where(codes < 0, C, codes), up)[:C]
+    status = torch.zeros(16, dtype=torch.int32, device=DEV)
+    status[1], status[3] = N.DEVERR_BOUNDS, 9
+    before = status.clone()
+    size = L.gsb_codebook_backward_workspace_size(n, 1, C, 1)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    ws = [torch.full((size,), 255, dtype=torch.uint8, device=DEV) for _ in streams]
+    got = [[torch.full((C,), math.nan, device=DEV) for _ in range(6)] for _ in streams]
+    torch.cuda.synchronize()
+    for turn in range(6):
+        for s, w, out in zip(streams, ws, got):
+            rc = L.gsb_codebook_backward(0, 0, n, 1, C, 1, None, 1, codes.data_ptr(), 4, None, 1.0, up.data_ptr(),
+                                         out[turn].data_ptr(), None, status.data_ptr(), w.data_ptr(), size,
+                                         s.cuda_stream)
+            assert rc == 0
+    torch.cuda.synchronize()
+    for out in got:
+        for t in out:
+            assert torch.equal(t, ref)
+    assert torch.equal(status, before)
+
+
 # ---- the sources ---------------------------------------------------------------
 def test_local_arrays_read_wide_are_aligned():
     """A local array of narrow values that is read as one 16-byte (or 8-byte) value lies on such a boundary
