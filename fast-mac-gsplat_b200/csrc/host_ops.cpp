@@ -29,6 +29,7 @@
 #include <stdexcept>
 #include <tuple>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "gsplat_b200.h"
@@ -159,6 +160,16 @@ ErrorRing& errors() {
   return *r;
 }
 
+// The error that a status block in host memory holds, and its site; no error is left.
+// One exchange, since kernels and other host threads may be at the block too: what is
+// recorded during the call is either in the result or still there. The site is the
+// last recorded one and stays.
+std::pair<uint32_t, uint32_t> take_status_error(uint32_t* w) {
+  if (__atomic_load_n(&w[GSB_STATUS_ERROR], __ATOMIC_RELAXED) == 0) return {0u, 0u};
+  const uint32_t flags = __atomic_exchange_n(&w[GSB_STATUS_ERROR], 0u, __ATOMIC_ACQ_REL);
+  return {flags, __atomic_load_n(&w[GSB_STATUS_ERROR_SITE], __ATOMIC_RELAXED)};
+}
+
 // Status blocks of the codebook ops, one per device, in pinned host memory that
 // the kernels write through its mapping: an op needs no copy, event or side
 // stream for its errors, so it can be captured into a graph whose replays report
@@ -167,7 +178,7 @@ ErrorRing& errors() {
 struct MappedStatus {
   static constexpr int kMaxDevices = 64;
   std::mutex mu;
-  volatile uint32_t* words = nullptr;  // [kMaxDevices][GSB_STATUS_WORDS]
+  uint32_t* words = nullptr;  // [kMaxDevices][GSB_STATUS_WORDS]
   std::array<bool, kMaxDevices> used{};
 
   uint32_t* of(int dev) {
@@ -183,28 +194,28 @@ struct MappedStatus {
       cudaThreadExchangeStreamCaptureMode(&mode);
       if (e != cudaSuccess) throw std::runtime_error("gsplat_b200: no pinned host memory for the status blocks");
       std::memset(p, 0, bytes);
-      words = static_cast<volatile uint32_t*>(p);
+      words = static_cast<uint32_t*>(p);
     }
     used[dev] = true;
-    return const_cast<uint32_t*>(words) + dev * GSB_STATUS_WORDS;  // unified addressing: the device's address too
+    return words + dev * GSB_STATUS_WORDS;  // unified addressing: the device's address too
+  }
+  // The block of a device, or nullptr where no op has had it.
+  uint32_t* given(int dev) {
+    std::lock_guard<std::mutex> g(mu);
+    return used[dev] ? words + dev * GSB_STATUS_WORDS : nullptr;
   }
   // Raises, once, an error that a finished kernel of the device has recorded.
-  void check(int dev) {
-    if (words == nullptr) return;
-    volatile uint32_t* w = words + dev * GSB_STATUS_WORDS;
-    const uint32_t flags = w[GSB_STATUS_ERROR];
-    if (!flags) return;
-    const uint32_t site = w[GSB_STATUS_ERROR_SITE];
-    w[GSB_STATUS_ERROR] = 0;
-    w[GSB_STATUS_ERROR_SITE] = 0;
-    throw std::runtime_error(decode_device_error(flags, site));
+  static void check(uint32_t* block) {
+    const auto [flags, site] = take_status_error(block);
+    if (flags) throw std::runtime_error(decode_device_error(flags, site));
   }
   void check_all() {
     for (int d = 0; d < kMaxDevices; ++d) {
-      if (!used[d]) continue;
+      uint32_t* const block = given(d);
+      if (block == nullptr) continue;
       const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(d));
       C10_CUDA_CHECK(cudaDeviceSynchronize());
-      check(d);
+      check(block);
     }
   }
 };
@@ -761,9 +772,8 @@ int32_t code_bytes(const Tensor& codes) { return codes.scalar_type() == at::kLon
 
 // A status block for the op's kernels; raises what earlier ones have recorded.
 uint32_t* codebook_status(const Tensor& t) {
-  const int dev = t.device().index();
-  uint32_t* s = mapped_status().of(dev);
-  mapped_status().check(dev);
+  uint32_t* s = mapped_status().of(t.device().index());
+  MappedStatus::check(s);
   return s;
 }
 // Under GSPLAT_B200_CHECK the op waits for its own errors (not in a capture).
@@ -774,7 +784,7 @@ void codebook_done(const Tensor& t) {
   C10_CUDA_CHECK(cudaStreamIsCapturing(cur.stream(), &capturing));
   if (capturing != cudaStreamCaptureStatusNone) return;
   cur.synchronize();
-  mapped_status().check(t.device().index());
+  MappedStatus::check(mapped_status().of(t.device().index()));
 }
 
 // Sizes that the kernels take as 32-bit numbers.
@@ -1215,6 +1225,7 @@ TORCH_LIBRARY_IMPL(gsplat_b200, CUDA, m) {
 PYBIND11_MODULE(_gsb_host, m) {
   m.doc() = "Native host runtime of the B200 rasterizer autograd path (drives the C ABI).";
   m.def("check_device_errors", &check_device_errors);
+  m.def("take_status_error", [](uintptr_t block) { return take_status_error(reinterpret_cast<uint32_t*>(block)); });
   m.def("codebook_lookup", &codebook_lookup);
   m.def("code_log_probs", &code_log_probs);
   m.def("code_balance_loss", &code_balance_loss);

@@ -12,8 +12,13 @@ no others).
 """
 from __future__ import annotations
 
+import ctypes
+import itertools
 import math
+import multiprocessing
 import re
+import time
+from multiprocessing.shared_memory import SharedMemory
 from pathlib import Path
 
 import pytest
@@ -22,7 +27,7 @@ import torch
 import torch_gsplat_bridge_fast as tgb
 from oracle import torch_ref as TR
 from torch_gsplat_bridge_fast import _native as N
-from torch_gsplat_bridge_fast.rasterize import _ops
+from torch_gsplat_bridge_fast.rasterize import _host, _ops
 
 U = 2.0**-24
 REL_EXP = 128 * U + 4 * U
@@ -133,6 +138,68 @@ def test_c_entries_refuse_before_any_launch():
         L.gsb_code_balance_backward(0, 4, 8, z, 8, st, state, g, dz, None)
     for bad in (dict(z=None), dict(st=None), dict(state=None), dict(g=None), dict(dz=None)):
         assert bb(**bad) == 1, bad
+
+
+def _record_errors(name):
+    """Two errors in a row for each number that the reader puts into word 8, then that number in word 9."""
+    shm = SharedMemory(name)
+    w = memoryview(shm.buf).cast("I")
+    try:
+        done = w[9] = 0xFFFFFFFF
+        while (t := w[8]) != 0xFFFFFFFF:
+            if t == done:
+                continue
+            for _ in range(t % 50):  # at any time
+                pass
+            w[3], w[1] = 9, 2 * t & 0xFFFFFFFF
+            w[3], w[1] = 9, 2 * t + 1 & 0xFFFFFFFF
+            w[9] = done = t
+    finally:
+        w.release()
+        shm.close()
+
+
+def test_errors_recorded_while_others_are_read_are_not_lost():
+    """What a kernel writes into the status words while the host takes an earlier error is in that result or in
+    the next. The kernel is another process here, the mapped words shared memory."""
+    take = _host().take_status_error
+    shm = SharedMemory(create=True, size=64)
+    w = memoryview(shm.buf).cast("I")
+    probe = ctypes.c_char.from_buffer(shm.buf)
+    address = ctypes.addressof(probe)
+    writer = multiprocessing.get_context("spawn").Process(target=_record_errors, args=(shm.name,), daemon=True)
+    lost = t = 0
+    try:
+        for i in range(16):
+            w[i] = 0
+        w[8] = 0xFFFFFFFE  # a number to begin with: the writer is there once it has answered
+        assert take(address) == (0, 0)
+        writer.start()
+        while w[9] != 0xFFFFFFFE:
+            assert writer.is_alive()
+        assert take(address) == (0xFFFFFFFD, 9)
+        stop = time.monotonic() + 4.0
+        while time.monotonic() < stop:
+            t += 1
+            w[8], last, done = t, 0, False
+            for turn in itertools.count(1):
+                assert turn % 65536 or writer.is_alive()
+                flags, site = take(address)
+                if flags:
+                    assert site == 9
+                    last = flags
+                elif done:
+                    break
+                done = w[9] == t
+            lost += last != 2 * t + 1
+    finally:
+        w[8] = 0xFFFFFFFF
+        writer.join(60)
+        w.release()
+        del probe
+        shm.close()
+        shm.unlink()
+    assert t > 0 and lost == 0
 
 
 # ---- the 64-bit restatements themselves, against differences --------------------
