@@ -1113,6 +1113,46 @@ def test_lookup_gradient_beside_errors_of_other_calls():
     assert torch.equal(status, before)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [48, 27, 300, 400])
+@pytest.mark.parametrize("bag", [0, 2])
+@pytest.mark.parametrize("kind", ["one code", "two codes", "sorted", "even"])
+def test_lookup_gradients_of_much_used_codes_are_exact(dtype, dim, bag, kind):
+    """Runs that cross stretches and blocks, in rows of whole pieces, odd rows and rows of two tiles: small
+    whole numbers, whose sums (below 2^24) are exact in any order and are rounded once to the result's type. A
+    block that is left out or counted twice shows in every column."""
+    rows, C = (70001, 300) if dim < 300 else (20011, 40)
+    g = _gen(dim + bag)
+    shape = (rows, bag) if bag else (rows,)
+    codes = torch.randint(0, C, shape, device=DEV, generator=g)
+    if kind == "one code":
+        codes.fill_(C - 1)
+    elif kind == "two codes":
+        codes.fill_(3)[rows // 3 :] = 4
+    elif kind == "sorted":
+        codes = codes.reshape(-1).sort().values.reshape(shape)
+    codes[torch.rand(shape, device=DEV, generator=g) < 0.1] = -1
+    whole = lambda lo, hi, *s: torch.randint(lo, hi + 1, s, device=DEV, generator=g).float()
+    table = whole(-3, 3, C, dim).to(dtype).requires_grad_(True)
+    w = whole(-2, 2, *shape).requires_grad_(True) if bag else None
+    up = whole(1, 4, rows, dim)  # of one sign: sums that nothing cancels
+    out = tgb.codebook_lookup(table, codes, w, out_dtype=torch.float32)
+    T = table.detach().double()
+    cc = codes.reshape(rows, -1)
+    ww = (w.detach() if bag else torch.ones(rows, 1, device=DEV)).double() * (cc >= 0)
+    picked = T[cc.clamp(min=0)]
+    assert torch.equal(out.detach().double(), (picked * ww[..., None]).sum(1))
+    grads = torch.autograd.grad(out, (table, w) if bag else (table,), up)
+    ref = torch.zeros(C, dim, device=DEV, dtype=torch.float64)
+    for j in range(cc.shape[1]):
+        ref.index_add_(0, cc[:, j].clamp(min=0), up.double() * ww[:, j, None])
+    assert ref.abs().max() < 2**24
+    assert torch.equal(grads[0], ref.to(dtype))
+    if bag:
+        assert torch.equal(grads[1].double(), (picked * up.double()[:, None]).sum(-1) * (cc >= 0))
+
+
 # ---- the sources ---------------------------------------------------------------
 def test_local_arrays_read_wide_are_aligned():
     """A local array of narrow values that is read as one 16-byte (or 8-byte) value lies on such a boundary
