@@ -183,9 +183,20 @@ def check(rc: int, what: str) -> None:
         raise NativeError(f"{what} failed with status {rc}: {msg}")
 
 
+class TensorAddress(int):
+    """The address of a tensor's values; keeps the tensor."""
+
+    tensor: torch.Tensor
+
+
 def ptr(t: torch.Tensor | None):
-    """Device pointer of a tensor as an int (None -> NULL)."""
-    return None if t is None else t.data_ptr()
+    """Device pointer of a tensor as an int (None -> NULL). The int keeps the tensor, so that of a temporary,
+    `ptr(x.to(device))`, the memory is not given to the next allocation before the call that it is an argument of."""
+    if t is None:
+        return None
+    address = TensorAddress(t.data_ptr())
+    address.tensor = t
+    return address
 
 
 def stream_ptr(device: torch.device):

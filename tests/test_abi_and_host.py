@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes as C
 import re
+import weakref
 from pathlib import Path
 
 import pytest
@@ -275,3 +276,18 @@ def test_fast_division_by_invariant_matches_integer_division():
         assert int(s.max()) < 2 ** 32
         q = s >> np.uint64(shift)
         assert np.array_equal(q, n // np.uint64(d)), d
+
+
+def test_the_pointer_of_a_temporary_keeps_its_memory():
+    """ptr(x.to(device)) as an argument: the tensor lives until the call returns, so that the next argument's
+    tensor does not get its memory."""
+    t = torch.arange(4.0)
+    alive = weakref.ref(t)
+    address = t.data_ptr()
+    p = N.ptr(t)
+    del t
+    assert alive() is not None and isinstance(p, int) and p == address and N.ptr(None) is None
+    seen = C.CFUNCTYPE(C.c_size_t, C.c_void_p)(lambda q: q)
+    assert seen(p) == address and C.c_void_p.from_param(p) is not None
+    del p
+    assert alive() is None
