@@ -5,9 +5,10 @@
 // columns are needed: with the counts at hand each row is one weighted softmax sum
 // (code_rows.cuh), read once. The sums of d over rows are 64-bit, in a fixed order.
 //
-// Forward and backward, of these the pass over the rows: 2^20 x 256 bf16 335 and 139 us
-// (3.9 TB/s; instructions, of which a count a value), 16,384 x 16,383 fp16 468 and 190,
-// 65,536 x 1,000 fp32 forward alone 64 and 55 (4.8 TB/s).
+// Forward and backward, of these the pass over the rows: 2^20 x 256 bf16 335 to 342 and
+// 139 us (3.9 TB/s), 16,384 x 16,383 fp16 468 and 190, 65,536 x 1,000 fp32 forward alone 64
+// and 55 (4.8 TB/s). What holds the pass over the rows is latency: 46 to 58 % of the issue
+// slots with the 22 to 35 % of the warps that its registers leave.
 #include "code_tiles.cuh"
 
 namespace gsb {
@@ -30,6 +31,9 @@ __host__ __device__ inline int64_t padded(int64_t codes) { return (codes + 7) / 
 __host__ __device__ inline Counts counts_of(const float* state, int64_t codes) {
   return Counts{state + kStateHead, state + kStateHead + padded(codes), padded(codes) / 8};
 }
+// From 2^24 uses of one code on its count is rounded to fp32, by 2^-24 of it at most, and so
+// are differences of such counts, whatever their own size. A 64-bit count would cost a value
+// twice the bytes and its half of a packed operation.
 __device__ __forceinline__ void put_count(float* state, int64_t codes, int64_t c, float n) {
   state[kStateHead + c] = n;
   state[kStateHead + padded(codes) + (c & 7) * (padded(codes) / 8) + (c >> 3)] = n;
@@ -228,9 +232,10 @@ __global__ void __launch_bounds__(256)
 
 // dz_c = g coef p_c ((n_c - n_a) - dr); bound by the logits' and the gradient's bytes where
 // both are read in whole pieces: 16,384 x 4,096 fp32 79 us (its last writes still
-// in L2), 2^20 x 64 bf16 55 (5.1 TB/s); between 16-byte boundaries by instructions, a count being a load of its own:
-// 2,047 x 50,001 fp16 102 us (4.0 TB/s). `at` deals out the result's values (SAME: the
-// logits' lie alike), p and dz are their place 0, that of code -shift.
+// in L2), 2^20 x 64 bf16 55 (5.1 TB/s). Between 16-byte boundaries, where a count is a load
+// of its own and registers spill, 69 % of the issue slots: 2,047 x 50,001 fp16 102 us
+// (4.0 TB/s). `at` deals out the result's values (SAME: the logits' lie alike), p and dz are
+// their place 0, that of code -shift.
 template <bool SAME, typename T, Mode M>
 __device__ __forceinline__ void balance_grad(float k, float4 st, const Deal<T, M>& at, int shift, bool on,
                                              const T* __restrict__ p, const Counts& counts, T* __restrict__ dz) {

@@ -4,8 +4,9 @@
 // A -inf logit has probability 0. In a row of -inf only log p is -inf, H and the
 // gradient are 0. NaN or +inf make a row's results NaN.
 //
-// Forward and backward, of these the forward: 65,536 x 4,096 fp32 with 4 alternatives 560
-// and 230 us (4.7 TB/s), 2,047 x 50,001 fp16 156 and 55, 2^20 x 64 bf16 with 2 161 and 71.
+// Forward and backward, of these the forward: 65,536 x 4,096 fp32 with 4 alternatives 540
+// to 566 and 230 us (4.7 TB/s), 2,047 x 50,001 fp16 157 and 55, 2^20 x 64 bf16 with 2 162
+// and 71.
 #include "code_tiles.cuh"
 
 namespace gsb {
@@ -54,7 +55,8 @@ __device__ __forceinline__ uint64_t warp_max(uint64_t key) {
 
 // Alternatives of a row that L lanes have in `buf` (a slice holds it all), one by
 // one: every lane has its own largest, taken out of the buffer; the row's largest of
-// those is next, and its lane looks for another.
+// those is next, and its lane looks for another, through all its values again: 2^20 x 64
+// bf16, forward, with 2, 8, 16 and 32 alternatives 77, 131, 219 and 512 us.
 template <typename T, int L>
 __device__ __forceinline__ void pick_alternatives(const LaneBuf& buf, int lane, const TilePlace<T, L>& now,
                                                   const Slice<T, L>& at, const RowStat& own, const RowResult& q,
@@ -385,7 +387,10 @@ struct RowGrad {
   __device__ __forceinline__ float alpha() const { return (gh * st.z - lead) * inv; }
 };
 // The second writing of a place: alternative j, or (j = top_k) the given code where it
-// is none of the alternatives. Its loads can be made ahead.
+// is none of the alternatives. Its loads can be made ahead. Each place adds up the others'
+// gradients anew, k^2 loads a row, which shows from 16 alternatives on: 2, 8, 16 and 32
+// take 90, 211, 778 and 4,660 us at 2^20 x 64 bf16 (a lane a row), 61, 78, 113 and 385 at
+// 65,536 x 512 fp32.
 struct Special {
   int64_t c;  // -1: none
   float own, others, z;
@@ -503,7 +508,8 @@ __global__ void __launch_bounds__(kGroupThreads, kRowThreadsSM / kGroupThreads)
 
 // Longer rows: W warps a stretch of the result (SAME: the logits' rows lie alike).
 // 16,384 x 4,096 fp32: 92 us, 5.8 TB/s; 2,047 x 50,001 fp16, rows between 16-byte
-// boundaries, 105 us, 3.9 TB/s: half of the instruction slots.
+// boundaries, 105 us, 3.9 TB/s: half of the issue slots and a quarter of the DRAM rate, so
+// the latency of what a thread does in turn (16,384 x 16,383 fp16 342 us, x 16,384 261).
 template <typename T, Mode M, bool SAME, int W>
 __global__ void __launch_bounds__(W * 32, kRowThreadsSM / (W * 32))
     k_log_probs_bwd_block(int64_t items, int64_t C, int parts, int part_len, const T* __restrict__ logits,

@@ -16,7 +16,7 @@
 // Bound by the logits' bytes while a value costs no more than a few instructions: a
 // maximum and a minimum (of two values at a time for 16-bit types), a conversion, and
 // half of each of an FMA, an addition and an FMA on pairs around one ex2. What is reached
-// is below both bounds: half of the instruction slots and 55 to 60 % of nominal DRAM rate
+// is below both bounds: half of the issue slots and 55 to 60 % of nominal DRAM rate
 // with fp32, 27 to 33 % with 16-bit types, 4 or 6 blocks an SM (registers) hiding latency.
 #pragma once
 

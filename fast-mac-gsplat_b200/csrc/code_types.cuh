@@ -1,4 +1,5 @@
-// Element types and index types of the codebook kernels (codebook.cu, code_probs.cu).
+// Element types and index types of the codebook kernels (codebook.cu, code_log_probs.cu,
+// code_balance.cu).
 #pragma once
 
 #include <cuda_bf16.h>

@@ -55,7 +55,8 @@ __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&v)[V]
 // (kStage; they are each wanted by every piece of a row) unless rows are so short that
 // there are too many of them. Bound by the stores: the table comes from L2 and L1.
 // 2^20 rows of 48, fp16 to fp32: 41 us, 5.0 TB/s (two pieces 47, eight 51; a fill of the
-// result alone takes 30). Four of 27 bf16 for 100,003 rows: 13 us, bound by instructions.
+// result alone takes 30). Four of 27 bf16 for 100,003 rows: 13 us, 76 % of the issue slots
+// (one load a value).
 constexpr int kLookupItems = 4;
 constexpr int kLookupPieces = 256 * kLookupItems;  // a block's
 constexpr int kLookupSlots = 2048;                 // that are staged, at most
@@ -285,7 +286,8 @@ __global__ void __launch_bounds__(256, WGRAD ? 1 : 4)
     if (i >= 1 && i <= L) s_val[i - 1] = i <= cnt ? vals[k] : 0u;
   }
   if (given_up) {
-    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) put_error(status, GSB_DEVERR_LOOKBACK_TIMEOUT, kSiteSortLookback);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0)
+      put_error(status, GSB_DEVERR_LOOKBACK_TIMEOUT, kSiteSortLookback);
     return;
   }
   __syncthreads();
@@ -478,8 +480,10 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// One warp per slot, where rows are too long for one tile of k_run_sums. Bound by the two
-// rows it reads, from L2 as a rule: 2 of 1,200 fp32 for 20,000 rows 38 us, 10 TB/s.
+// One warp per slot: where rows are too long for one tile of k_run_sums, and where the
+// codebook has no gradient (a frozen one). Bound by the two rows it reads, from L2 as a rule:
+// 2 of 1,200 fp32 for 20,000 rows 38 us, 10 TB/s. Rows shorter than a warp leave lanes idle:
+// 4 of bf16 for 100,003 rows take 76 us with 27 values, 86 with 48, 139 with 400.
 template <typename T, typename O>
 __global__ void __launch_bounds__(256)
     k_weight_grad(int64_t slots, int bag, int64_t C, int dim, const T* __restrict__ table, int64_t stride, Codes codes,
